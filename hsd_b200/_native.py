@@ -19,6 +19,7 @@ HSD_MODE_NORMAL, HSD_MODE_SPEC, HSD_MODE_TREE, HSD_MODE_FINISHED = 0, 1, 2, 3
 HSD_DEV_TIMEOUT = 0x10000
 HSD_DEV_BAD_INDEX = 0x20000
 HSD_DEV_CAPACITY = 0x40000
+HSD_DEV_BAD_VALUE = 0x80000
 
 
 class HSDError(RuntimeError):
@@ -107,6 +108,11 @@ SIGNATURES = [
     ("hsd_rope_append", C.c_int,
      [_P, _I64, _P, _P, _I64, _P, _P, _I64, _I32, _I32, _I32, _I32, _P, _I64, _P, _I64, _I64,
       _I32, _P]),
+    ("hsd_rope_append_axes", C.c_int,
+     [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _I32, _P, _P, _F, _I32, _I32, _I32,
+      _I32, _P, _I64, _P, _I64, _I64, _I64, _P, _P]),
+    ("hsd_kv8_seal", C.c_int, [_P, _I32, _I64, _P, _I64, _P, _I64, _I32, _I32, _P, _P]),
+    ("hsd_kv8_unseal", C.c_int, [_P, _I64, _P, _I64, _I32, _I64, _I32, _P, _I64, _P]),
     ("hsd_continuation_trees", C.c_int,
      [_P, _P, _P, _P, _I32, _I32, _I32, _P, _P, _P, _P, _P, _P, _P]),
     ("hsd_selftest_bounded_wait", C.c_int, [_P, _P, _P]),

@@ -8,8 +8,15 @@ between the projections and the attention call
 the whole layer cache).  One launch rotates the query rows in place in the
 ``q_proj`` output and writes the rotated key rows and the value rows into
 preallocated cache planes; results are bit-identical to torch's bf16 ops.
+
+:func:`rope_append_axes` does the same for positions with several axes (image
+and video tokens; the HunYuan pipeline's four, H:2033), computing the angles
+from the position ids instead of reading tables.
 """
 from __future__ import annotations
+
+import math
+from fractions import Fraction
 
 import torch
 
@@ -74,3 +81,141 @@ def rope_append(q, k, v, cos, sin, k_cache, v_cache, dst_row0, num_q_heads=None,
     if q2 is None:
         return None
     return q2.unflatten(-1, (hq, 128)).unsqueeze(0).transpose(1, 2)
+
+
+# ---------------------------------------------------------------- several axes
+# 2 pi to 240 bits, as a fraction (the first digits of pi are public constants)
+_TWO_PI = Fraction("6.283185307179586476925286766559005768394338798750211641949889184615632812572"
+                   "417997256069650684234136")
+_MAX_AXES = 8
+
+
+class RotaryAxes:
+    """Frequencies of a rotary embedding whose 64 dimension pairs turn with
+    several position axes (time / height / width, or the four axes of the
+    HunYuan pipeline's ``[1, 4, Q]`` position ids, H:2033).
+
+    ``sections[a]``: how many pairs turn with axis ``a``; they sum to 64.  By
+    default the pairs are shared out in order (the first ``sections[0]`` pairs
+    turn with axis 0, and so on); with ``interleaved`` pair ``i`` turns with
+    axis ``i % A`` while ``i < A * sections[i % A]`` and with axis 0 beyond
+    (the later axes then need an equal share at most ``64 // A`` each).
+    ``theta``: pair ``i`` turns ``theta ** (-i / 64)`` rad per position, or
+    ``inv_freq`` gives the 64 frequencies (a model's buffer: its exact values
+    are used).  ``scaling`` multiplies the cosines and sines.
+
+    The device tables are made here, once; one object serves every layer.
+    """
+
+    def __init__(self, sections, theta=1e6, interleaved=False, inv_freq=None, scaling=1.0,
+                 device="cuda"):
+        self.sections = [int(n) for n in sections]
+        self.scaling = float(scaling)
+        axes = len(self.sections)
+        if not 1 <= axes <= _MAX_AXES or min(self.sections) < 0 or sum(self.sections) != 64:
+            raise ValueError(f"RotaryAxes: sections {self.sections} must be 1 to {_MAX_AXES} "
+                             "counts that sum to 64 pairs")
+        if interleaved:
+            axis = [i % axes if i < axes * self.sections[i % axes] else 0 for i in range(64)]
+            if [axis.count(a) for a in range(axes)] != self.sections:
+                raise ValueError(f"RotaryAxes: sections {self.sections} cannot be interleaved")
+        else:
+            axis = [a for a, n in enumerate(self.sections) for _ in range(n)]
+        if inv_freq is None:
+            if not (math.isfinite(theta) and theta > 0):
+                raise ValueError(f"RotaryAxes: theta {theta} must be positive")
+            freq = [float(theta) ** (-i / 64) for i in range(64)]
+        else:
+            freq = torch.as_tensor(inv_freq, dtype=torch.float64).reshape(-1).tolist()
+        if len(freq) != 64 or not all(math.isfinite(f) for f in freq):
+            raise ValueError("RotaryAxes: 64 finite frequencies are needed")
+        if not math.isfinite(self.scaling):
+            raise ValueError("RotaryAxes: scaling must be finite")
+        # turns per position in units of 2^-64 turn, modulo one turn
+        turns = [round(Fraction(f) / _TWO_PI * 2 ** 64) % 2 ** 64 for f in freq]
+        self.turns = torch.tensor([t - 2 ** 64 if t >= 2 ** 63 else t for t in turns],
+                                  dtype=torch.int64, device=device)
+        self.pair_axis = torch.tensor(axis, dtype=torch.int32, device=device)
+
+    @property
+    def axes(self):
+        return len(self.sections)
+
+
+def _positions(positions, axes, rows):
+    p = positions
+    if p.dim() == 3:  # [1, A, Q] or [A, 1, Q]
+        if p.shape[0] == 1:
+            p = p[0]
+        elif p.shape[1] == 1:
+            p = p[:, 0]
+    if p.dim() == 1 and axes == 1:
+        p = p[None]
+    if p.dim() != 2 or tuple(p.shape) != (axes, rows):
+        raise ValueError(f"rope_append_axes: positions {tuple(positions.shape)}, expected "
+                         f"[{axes}, {rows}]")
+    if p.dtype == torch.int32:
+        p = p.long()
+    if p.dtype != torch.int64 or not p.is_cuda:
+        raise TypeError("rope_append_axes: positions must be an int64 or int32 CUDA tensor")
+    return p
+
+
+def rope_append_axes(q, k, v, positions, rotary, k_cache, v_cache, dst_row0, out=None,
+                     num_q_heads=None, num_kv_heads=None, status=None):
+    """:func:`rope_append` for positions with several axes, without cos / sin
+    tables: the angles come from the integer ``positions``.
+
+    q, k, v, k_cache, v_cache, dst_row0 as in :func:`rope_append` (k and v may
+    have different row strides); positions: int64 ``[A, Q]`` (``[1, A, Q]`` and
+    ``[A, 1, Q]`` too; any strides, an expanded row included), any values;
+    rotary: the :class:`RotaryAxes` of the model.  The queries are rotated in
+    place, or into ``out`` (``[..., Q, Hq * 128]`` bf16, not overlapping q).
+    Arithmetic is fp32 with one rounding to bf16, with angles exact to fp32 at
+    any position (:func:`rope_append` reproduces torch's bf16 products).
+    Returns the rotated queries as a ``[1, Hq, Q, 128]`` view, or None when q
+    is None.  Asynchronous on the device's current stream.
+    """
+    kc, vc = _cache(k_cache, "k_cache"), _cache(v_cache, "v_cache")
+    hkv = num_kv_heads or kc.shape[0]
+    k2, v2 = _rows(k, "k", hkv * 128), _rows(v, "v", hkv * 128)
+    n = k2.shape[0]
+    if v2.shape[0] != n:
+        raise ValueError("rope_append_axes: k and v row counts differ")
+    if kc.stride() != vc.stride() or kc.shape != vc.shape or kc.shape[0] != hkv:
+        raise ValueError("rope_append_axes: k_cache and v_cache must have one layout")
+    if dst_row0 < 0 or dst_row0 + n > kc.shape[1]:
+        raise ValueError(f"rope_append_axes: rows {dst_row0}..{dst_row0 + n} past the cache")
+    pos = _positions(positions, rotary.axes, n)
+    hq, q2, o2 = 0, None, None
+    if q is not None:
+        hq = num_q_heads or q.shape[-1] // 128
+        q2 = _rows(q, "q", hq * 128)
+        o2 = q2 if out is None else _rows(out, "out", hq * 128)
+        if q2.shape[0] != n or o2.shape[0] != n:
+            raise ValueError("rope_append_axes: q, out and k row counts differ")
+        if out is not None and o2.data_ptr() != out.data_ptr():
+            raise ValueError("rope_append_axes: out must be rows of one stride")
+    elif out is not None:
+        raise ValueError("rope_append_axes: out without q")
+    dev = k2.device
+    tensors = (k2, v2, kc, vc, pos, rotary.turns, q2, o2)
+    if any(t is not None and t.device != dev for t in tensors):
+        raise ValueError("rope_append_axes: all tensors must be on one device")
+    if q2 is not None and out is None and q2.data_ptr() != q.data_ptr():
+        raise ValueError("rope_append_axes: q must be rows of one stride")
+    if kc.data_ptr() != k_cache.data_ptr() or vc.data_ptr() != v_cache.data_ptr():
+        raise ValueError("rope_append_axes: the caches must be views [..., Hkv, KV, 128]")
+    if n:
+        lib = N.load()
+        with torch.cuda.device(dev):
+            N.check(lib.hsd_rope_append_axes(
+                N.ptr(q2), 0 if q2 is None else q2.stride(0), N.ptr(o2),
+                0 if o2 is None else o2.stride(0), N.ptr(k2), k2.stride(0), N.ptr(v2),
+                v2.stride(0), N.ptr(pos), pos.stride(0), pos.stride(1), rotary.axes,
+                N.ptr(rotary.turns), N.ptr(rotary.pair_axis), rotary.scaling, n, hq, hkv, 128,
+                N.ptr(kc), kc.stride(0), N.ptr(vc), vc.stride(0), kc.stride(1), dst_row0,
+                N.ptr(status), N.stream_handle()), "hsd_rope_append_axes")
+    if q2 is None:
+        return None
+    return o2.unflatten(-1, (hq, 128)).unsqueeze(0).transpose(1, 2)

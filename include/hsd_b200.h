@@ -10,7 +10,8 @@
  * it after its next synchronisation.  Every device pointer is caller-owned.
  *
  * The step's kernels (tile plan, attention, KV append, RoPE + cache update,
- * acceptance + KMP, keep indices, compaction, bit remap) are launched with
+ * acceptance + KMP, keep indices, compaction, bit remap, and the 8-bit
+ * cache's sealing, unsealing and attention) are launched with
  * programmatic stream serialization: each waits for the previous work on the
  * stream to complete before touching memory and lets the next kernel be
  * scheduled early.  A caller's kernel that follows on the same stream with
@@ -45,6 +46,7 @@ typedef struct CUstream_st *hsd_stream_t;
 #define HSD_DEV_TIMEOUT 0x10000
 #define HSD_DEV_BAD_INDEX 0x20000
 #define HSD_DEV_CAPACITY 0x40000
+#define HSD_DEV_BAD_VALUE 0x80000 /* hsd_kv8_seal: an infinity or NaN among the rows */
 
 /* segment kinds: the intra-segment pattern over the segment's new columns */
 #define HSD_SEG_CAUSAL 0 /* speculative / prefill block: tril (D:1442-1447, RD:234-245) */
@@ -334,6 +336,54 @@ int hsd_rope_append(void *q, int64_t q_row_stride, const void *k, const void *v,
                     int32_t num_kv_heads, int32_t head_dim, void *k_cache,
                     int64_t k_cache_head_stride, void *v_cache, int64_t v_cache_head_stride,
                     int64_t cache_row_stride, int32_t dst_row0, hsd_stream_t stream);
+
+/* Rotary embedding with several position axes + cache update, one launch; no
+ * tables: the angles come from the integer positions.  positions[a][r] (int64
+ * at element strides pos_axis_stride, pos_row_stride; 0 repeats one row for
+ * several axes): row r's position on axis a < n_axes (1 to 8), as the HunYuan
+ * loop's [1, 4, Q] ids (H:2033, H:2100, H:2128).  Pair i (dims i and i + 64)
+ * turns with axis pair_axis[i] at turns[i] = inv_freq[i] / 2 pi turns per
+ * position, in units of 2^-64 turn (modulo 1; device arrays of 64):
+ *   y_i = scaling (x_i cos - x_{i+64} sin),
+ *   y_{i+64} = scaling (x_{i+64} cos + x_i sin),
+ * computed in fp32 and rounded once to bf16 (hsd_rope_append rounds each
+ * product, as torch's bf16 ops do).  q, k, v: [n_rows][heads * 128] bf16 at
+ * their row strides; rotated queries go to q_out (q itself, or memory that
+ * does not overlap it), rotated keys and the values to cache rows
+ * [dst_row0, dst_row0 + n_rows).  num_q_heads may be 0.  A pair_axis outside
+ * [0, n_axes) sets HSD_DEV_BAD_INDEX and leaves that pair unturned.  Strides
+ * in elements, multiples of 8 (positions: any); bf16 pointers 16-byte aligned. */
+int hsd_rope_append_axes(const void *q, int64_t q_row_stride, void *q_out,
+                         int64_t q_out_row_stride, const void *k, int64_t k_row_stride,
+                         const void *v, int64_t v_row_stride, const int64_t *positions,
+                         int64_t pos_axis_stride, int64_t pos_row_stride, int32_t n_axes,
+                         const uint64_t *turns, const int32_t *pair_axis, float scaling,
+                         int32_t n_rows, int32_t num_q_heads, int32_t num_kv_heads,
+                         int32_t head_dim, void *k_cache, int64_t k_cache_head_stride,
+                         void *v_cache, int64_t v_cache_head_stride, int64_t cache_row_stride,
+                         int64_t dst_row0, int32_t *status, hsd_stream_t stream);
+
+/* ---- 8-bit KV cache ------------------------------------------------------- */
+
+/* No counterpart in the reference.  Seal n_blocks whole blocks of 64 rows of
+ * every plane (one layer's K or V of one KV head; rows of 128 bf16, 256
+ * contiguous bytes, plane addresses in src_planes as for hsd_compact_kv) from
+ * row src_row0 on.  Plane p's values go to data + p * plane_stride bytes
+ * (rows of 128 int8) from row 64 * block0 on, its scales to
+ * scale + p * scale_stride from entry block0 on:
+ *   a = max |x| of the block's finite values, at least 2^-100;
+ *   scale = a / 127; n = 127 x / a to the nearest, ties to even; x ~ n * scale.
+ * Infinities saturate, NaN becomes 0, and either sets HSD_DEV_BAD_VALUE.
+ * data and the planes 16-byte aligned, plane_stride a multiple of 16. */
+int hsd_kv8_seal(const uint64_t *src_planes, int32_t n_planes, int64_t src_row0, int8_t *data,
+                 int64_t plane_stride, float *scale, int64_t scale_stride, int32_t block0,
+                 int32_t n_blocks, int32_t *status, hsd_stream_t stream);
+
+/* Sealed rows [row0, row0 + n_rows) of every plane back as bf16 rows
+ * (n * scale, rounded once) to rows dst_row0.. of the planes dst_planes. */
+int hsd_kv8_unseal(const int8_t *data, int64_t plane_stride, const float *scale,
+                   int64_t scale_stride, int32_t n_planes, int64_t row0, int32_t n_rows,
+                   const uint64_t *dst_planes, int64_t dst_row0, hsd_stream_t stream);
 
 /* ---- (3) acceptance + KMP re-alignment ----------------------------------- */
 
