@@ -113,6 +113,10 @@ SIGNATURES = [
       _I32, _P, _I64, _P, _I64, _I64, _I64, _P, _P]),
     ("hsd_kv8_seal", C.c_int, [_P, _I32, _I64, _P, _I64, _P, _I64, _I32, _I32, _P, _P]),
     ("hsd_kv8_unseal", C.c_int, [_P, _I64, _P, _I64, _I32, _I64, _I32, _P, _I64, _P]),
+    ("hsd_kv8_attention_workspace_bytes", _SZ, [_I32, _I32, _I32, _I32]),
+    ("hsd_verify_attention_kv8", C.c_int,
+     [_P, _I64, _I64, _P, _I64, _P, _I64, _P, _P, _I64, _I32, _P, _I64, _I64, _P, _I64, _I64,
+      _I32, _P, _P, _I32, _I32, _I32, _I32, _I32, _F, C.POINTER(Plan), _P, _SZ, _P, _P]),
     ("hsd_continuation_trees", C.c_int,
      [_P, _P, _P, _P, _I32, _I32, _I32, _P, _P, _P, _P, _P, _P, _P]),
     ("hsd_selftest_bounded_wait", C.c_int, [_P, _P, _P]),

@@ -385,6 +385,33 @@ int hsd_kv8_unseal(const int8_t *data, int64_t plane_stride, const float *scale,
                    int64_t scale_stride, int32_t n_planes, int64_t row0, int32_t n_rows,
                    const uint64_t *dst_planes, int64_t dst_row0, hsd_stream_t stream);
 
+/* hsd_verify_attention over a cache whose columns [0, sealed) are held in 8
+ * bits (hsd_kv8_seal; sealed a multiple of 64) and whose columns
+ * [sealed, kv_len) are bf16: column c is row c - tail_row0 of k_tail / v_tail
+ * (tail_row0 = 0: a full cache whose sealed rows are not read;
+ * tail_row0 = sealed: the rows behind the sealed ones alone).  k8, v8: int8
+ * rows of 128 contiguous bytes, heads at the given byte strides; k_scale,
+ * v_scale: one per 64 rows, heads scale_head_stride apart.  Either side may
+ * be empty, its pointers then NULL.  The mask, out, lse and the strides of q
+ * and the tails are those of hsd_verify_attention; fully masked rows give 0
+ * and -inf, and what stands in a bf16 column that no query row of the tile
+ * sees does not matter.  P is rounded to bf16, everything else is fp32.
+ * workspace: hsd_kv8_attention_workspace_bytes, 256-byte aligned, zero-filled
+ * before its first use; each call leaves it ready for the next, and calls
+ * sharing one must not overlap in time. */
+size_t hsd_kv8_attention_workspace_bytes(int32_t q_len, int32_t kv_len, int32_t num_q_heads,
+                                         int32_t num_kv_heads);
+int hsd_verify_attention_kv8(const void *q, int64_t q_row_stride, int64_t q_head_stride,
+                             const int8_t *k8, int64_t k8_head_stride, const int8_t *v8,
+                             int64_t v8_head_stride, const float *k_scale, const float *v_scale,
+                             int64_t scale_head_stride, int32_t sealed, const void *k_tail,
+                             int64_t kt_row_stride, int64_t kt_head_stride, const void *v_tail,
+                             int64_t vt_row_stride, int64_t vt_head_stride, int32_t tail_row0,
+                             void *out, float *lse, int32_t q_len, int32_t kv_len,
+                             int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                             float scale, const hsd_plan_t *plan, void *workspace,
+                             size_t workspace_bytes, int32_t *status, hsd_stream_t stream);
+
 /* ---- (3) acceptance + KMP re-alignment ----------------------------------- */
 
 /* One warp per block: acceptance by mode (D:1107-1293, H:1633-1858 at
