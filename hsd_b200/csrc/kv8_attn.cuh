@@ -43,7 +43,10 @@ __device__ __forceinline__ void bytes_to_bf16(uint32_t w, uint32_t& lo, uint32_t
 }  // namespace hsd
 
 namespace hsd_host {
-// The two kernels behind hsd_verify_attention_kv8.
+// The two kernels behind hsd_verify_attention_kv8.  The workspace starts with
+// kKv8FlagBytes of flags and counters, zero before the first use and left
+// ready by every call; partial rows follow, in no state that a call relies on.
+constexpr size_t kKv8FlagBytes = 65536;
 struct Kv8AttnArgs {
   hsd::kv8a::Params p;
   const int8_t* k8;
@@ -57,6 +60,8 @@ struct Kv8AttnArgs {
 };
 size_t kv8_rows_workspace_bytes(int q_len, int kv_len, int hq, int hkv);
 int kv8_rows_launch(const Kv8AttnArgs& a);
+size_t kv8_tiles_workspace_bytes();
+int kv8_tiles_launch(const Kv8AttnArgs& a, const hsd_plan_t& plan);
 // 3-D map {128 dims, rows, heads} of int8 (box 128 x box_rows) or bf16 (box
 // 64 x box_rows), 128-byte swizzle.
 int kv8_map(CUtensorMap* map, const void* base, bool bf16, int64_t rows, int heads,

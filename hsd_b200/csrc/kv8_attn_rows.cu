@@ -512,8 +512,8 @@ int n_splits(int q_len, int kv_len, int hq, int hkv) {
 
 size_t kv8_rows_workspace_bytes(int q_len, int kv_len, int hq, int hkv) {
   const int s = n_splits(q_len, kv_len, hq, hkv);
-  if (s == 1) return 0;
-  return size_t(n_tiles(q_len, hq / hkv)) * hkv * s * kv8r::kRecord * sizeof(float);
+  if (s == 1) return kKv8FlagBytes;
+  return kKv8FlagBytes + size_t(n_tiles(q_len, hq / hkv)) * hkv * s * kv8r::kRecord * sizeof(float);
 }
 
 int kv8_map(CUtensorMap* map, const void* base, bool bf16, int64_t rows, int heads,
@@ -578,7 +578,8 @@ int kv8_rows_launch(const Kv8AttnArgs& a) {
   kv8r::Split sp;
   sp.n_tiles = n_tiles(p.q_len, p.group);
   sp.splits = n_splits(p.q_len, p.kv_len, p.hq, p.hkv);
-  sp.partials = sp.splits > 1 ? static_cast<float*>(a.workspace) : nullptr;
+  sp.partials = sp.splits > 1 ? reinterpret_cast<float*>(static_cast<char*>(a.workspace) + kKv8FlagBytes)
+                               : nullptr;
   if (sp.n_tiles > 65535 || p.hkv > 65535) {
     set_error("hsd_verify_attention_kv8: %d rows x %d heads exceed the launch's range", p.q_len,
               p.hq);

@@ -122,15 +122,19 @@ class Kv8Cache:
 
 
 _workspaces = {}
+_FLAG_BYTES = 65536  # leading part of the workspace that starts as zeros
 
 
 def _workspace(need, device):
-    """Zero-filled scratch of (device, current stream), grown to fit; every
-    call leaves it ready for the next.  A call that is being captured into a
-    graph gets scratch of its own, so graphs that share no stream share no
-    scratch either (replays of one graph never overlap)."""
+    """Scratch of (device, current stream), grown to fit; its flags are zeroed
+    once and every call leaves them ready for the next.  A call that is being
+    captured into a graph gets scratch of its own, zeroed by the graph, so
+    graphs that share no stream share no scratch either (replays of one graph
+    never overlap)."""
     if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(need + 256, dtype=torch.uint8, device=device)
+        buf = torch.empty(need + 256, dtype=torch.uint8, device=device)
+        buf[:_FLAG_BYTES + 256].zero_()
+        return buf
     key = (device.index, int(torch.cuda.current_stream(device).cuda_stream))
     buf = _workspaces.get(key)
     if buf is None or buf.numel() < need + 256:

@@ -396,9 +396,10 @@ int hsd_kv8_unseal(const int8_t *data, int64_t plane_stride, const float *scale,
  * and the tails are those of hsd_verify_attention; fully masked rows give 0
  * and -inf, and what stands in a bf16 column that no query row of the tile
  * sees does not matter.  P is rounded to bf16, everything else is fp32.
- * workspace: hsd_kv8_attention_workspace_bytes, 256-byte aligned, zero-filled
- * before its first use; each call leaves it ready for the next, and calls
- * sharing one must not overlap in time. */
+ * workspace: hsd_kv8_attention_workspace_bytes, 256-byte aligned, its first
+ * 64 KB zero-filled before the first use; each call leaves it ready for the
+ * next (after an error status, zero them again), and calls sharing one must
+ * not overlap in time. */
 size_t hsd_kv8_attention_workspace_bytes(int32_t q_len, int32_t kv_len, int32_t num_q_heads,
                                          int32_t num_kv_heads);
 int hsd_verify_attention_kv8(const void *q, int64_t q_row_stride, int64_t q_head_stride,
