@@ -9,8 +9,6 @@ bool strides_ok(const void* p, int64_t rs, int64_t hs) {
          (hs % 8) == 0;
 }
 
-bool use_rows(int32_t q_len, int32_t group) { return int64_t(q_len) * group <= 256; }
-
 }  // namespace
 
 extern "C" size_t hsd_kv8_attention_workspace_bytes(int32_t q_len, int32_t kv_len,
@@ -18,9 +16,7 @@ extern "C" size_t hsd_kv8_attention_workspace_bytes(int32_t q_len, int32_t kv_le
   if (q_len <= 0 || kv_len <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 ||
       num_q_heads % num_kv_heads)
     return 0;
-  if (use_rows(q_len, num_q_heads / num_kv_heads))
-    return hsd_host::kv8_rows_workspace_bytes(q_len, kv_len, num_q_heads, num_kv_heads);
-  return hsd_host::kv8_tiles_workspace_bytes();
+  return hsd_host::kv8_rows_workspace_bytes(q_len, kv_len, num_q_heads, num_kv_heads);
 }
 
 extern "C" int hsd_verify_attention_kv8(
@@ -106,6 +102,5 @@ extern "C" int hsd_verify_attention_kv8(
   a.vt_head_stride = vt_head_stride;
   a.workspace = workspace;
   a.stream = reinterpret_cast<cudaStream_t>(stream);
-  return use_rows(q_len, p.group) ? hsd_host::kv8_rows_launch(a)
-                                  : hsd_host::kv8_tiles_launch(a, *plan);
+  return hsd_host::kv8_rows_launch(a);
 }

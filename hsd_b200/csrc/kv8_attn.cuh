@@ -60,8 +60,6 @@ struct Kv8AttnArgs {
 };
 size_t kv8_rows_workspace_bytes(int q_len, int kv_len, int hq, int hkv);
 int kv8_rows_launch(const Kv8AttnArgs& a);
-size_t kv8_tiles_workspace_bytes();
-int kv8_tiles_launch(const Kv8AttnArgs& a, const hsd_plan_t& plan);
 // 3-D map {128 dims, rows, heads} of int8 (box 128 x box_rows) or bf16 (box
 // 64 x box_rows), 128-byte swizzle.
 int kv8_map(CUtensorMap* map, const void* base, bool bf16, int64_t rows, int heads,
