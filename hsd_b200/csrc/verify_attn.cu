@@ -538,9 +538,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int k = 0; k < 8; ++k) mx8[k] = x[k];
 #pragma unroll
-        for (int i = 8; i < 128; i += 16)
+        for (int i = 8; i + 16 <= 128; i += 16)
 #pragma unroll
           for (int k = 0; k < 8; ++k) mx8[k] = fmax3(mx8[k], x[i + k], x[i + 8 + k]);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) mx8[k] = fmaxf(mx8[k], x[120 + k]);
         const float mx = fmax3(fmax3(mx8[0], mx8[1], mx8[2]), fmax3(mx8[3], mx8[4], mx8[5]),
                                fmaxf(mx8[6], mx8[7]));
         const float m_new = fmaxf(m, mx * p.scale_log2);
