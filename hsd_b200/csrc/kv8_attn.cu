@@ -1,8 +1,207 @@
 // Packed verification attention over a cache whose first columns are held in
-// 8 bits: argument checks and the choice of kernel.
+// 8 bits: argument checks, the choice of kernel, and the path for many rows.
+//
+// Many rows.  Every K and V element meets every query tile and head pair (17 x
+// 3 times for a region page), so converting where it is used costs far more
+// than the cache's bytes; here one launch expands the layer's columns into
+// the workspace -- int8 to the same integers in bf16, exactly, the bf16 tail
+// copied behind them -- and the tcgen05 verification kernel (verify_attn.cu)
+// reads that, with one score factor and one V factor per 64 columns in its
+// softmax.  The expansion is bound by HBM and L2: 1 byte read and 2 written per
+// sealed value, and the attention finds it in L2.
 #include "kv8_attn.cuh"
+#include "verify_attn.cuh"
+
+namespace hsd {
+namespace kv8a {
+
+struct ExpandParams {
+  const int8_t* x8[2];  // K, V
+  int64_t head_stride8[2];
+  const float* scale[2];
+  int64_t scale_stride;
+  const __nv_bfloat16* tail[2];
+  int64_t row_stride[2], head_stride[2];
+  const uint8_t* tile_class;
+  const uint64_t* mask_words;
+  __nv_bfloat16* dst;  // [2][hkv][kv_len][128]
+  attn::ColumnScale* col_scale;
+  int kv_len, hkv, n_kv64, n_qtiles, sealed, tail_row0;
+  float scale_log2;
+};
+
+constexpr int kExpandThreads = 256;
+
+// Columns of a 64-column tile that some query row sees.
+__device__ __forceinline__ uint64_t seen_columns(const ExpandParams& p, int t, uint32_t* red) {
+  if (threadIdx.x < 2) red[threadIdx.x] = 0u;
+  __syncthreads();
+  uint64_t w = 0ull;
+  for (int i = threadIdx.x; i < p.n_qtiles * 128; i += kExpandThreads) {
+    const size_t tile = size_t(i >> 7) * p.n_kv64 + t;
+    const int cls = p.tile_class[tile];
+    if (cls == 2) w = ~0ull;
+    if (cls == 1) w |= p.mask_words[tile * 128 + (i & 127)];
+  }
+  const uint32_t lo = __reduce_or_sync(0xffffffffu, uint32_t(w));
+  const uint32_t hi = __reduce_or_sync(0xffffffffu, uint32_t(w >> 32));
+  if (lane_id() == 0) {
+    atomicOr(&red[0], lo);
+    atomicOr(&red[1], hi);
+  }
+  __syncthreads();
+  return uint64_t(red[0]) | (uint64_t(red[1]) << 32);
+}
+
+// CTA (64-column tile, KV head, K or V)
+__global__ void __launch_bounds__(kExpandThreads) expand_kernel(const ExpandParams p) {
+  pdl_wait_then_release();  // launched with launch_pdl
+  __shared__ uint32_t red[2];
+  const int t = blockIdx.x, h = blockIdx.y, z = blockIdx.z, tid = threadIdx.x;
+  const int col0 = 64 * t;
+  uint4* dst = reinterpret_cast<uint4*>(
+      p.dst + (size_t(z * p.hkv + h) * p.kv_len + col0) * HD);
+  if (col0 < p.sealed) {
+    const uint4* src =
+        reinterpret_cast<const uint4*>(p.x8[z] + h * p.head_stride8[z] + int64_t(col0) * HD);
+    uint4 v[2];
+    v[0] = __ldcs(src + tid);
+    v[1] = __ldcs(src + tid + kExpandThreads);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      uint32_t o[8];
+      bytes_to_bf16(v[u].x, o[0], o[1]);
+      bytes_to_bf16(v[u].y, o[2], o[3]);
+      bytes_to_bf16(v[u].z, o[4], o[5]);
+      bytes_to_bf16(v[u].w, o[6], o[7]);
+      const int at = 2 * (tid + u * kExpandThreads);
+      dst[at] = make_uint4(o[0], o[1], o[2], o[3]);
+      dst[at + 1] = make_uint4(o[4], o[5], o[6], o[7]);
+    }
+  } else {
+    // what stands in columns that no row sees must not reach the sums (0 * V)
+    const uint64_t seen = z == 1 ? seen_columns(p, t, red) : ~0ull;
+    const __nv_bfloat16* src = p.tail[z] + h * p.head_stride[z] +
+                               int64_t(col0 - p.tail_row0) * p.row_stride[z] + (tid & 15) * 8;
+    const int rows = min(64, p.kv_len - col0);
+    uint4 v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int r = 16 * u + (tid >> 4);
+      v[u] = make_uint4(0u, 0u, 0u, 0u);
+      if (r < rows && ((seen >> r) & 1ull))
+        v[u] = __ldg(reinterpret_cast<const uint4*>(src + r * p.row_stride[z]));
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int r = 16 * u + (tid >> 4);
+      if (r < rows) dst[r * 16 + (tid & 15)] = v[u];
+    }
+  }
+  if (z == 0 && tid == 0) {
+    float ks = 1.f, vs = 1.f;
+    if (col0 < p.sealed) {
+      ks = p.scale[0][h * p.scale_stride + t];
+      vs = p.scale[1][h * p.scale_stride + t];
+    }
+    attn::ColumnScale c;
+    c.score = ks * p.scale_log2;
+    c.log2_v = log2f(vs);
+    c.inv_v = 1.f / vs;
+    c.pad = 0.f;
+    attn::ColumnScale* dst_scale = p.col_scale + size_t(h) * ((p.n_kv64 + 1) & ~1) + t;
+    dst_scale[0] = c;
+    // the absent second half of an odd last block: any finite factors
+    if (t == p.n_kv64 - 1 && (t & 1) == 0) dst_scale[1] = {1.f, 0.f, 1.f, 0.f};
+  }
+}
+
+}  // namespace kv8a
+}  // namespace hsd
 
 namespace {
+
+size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
+
+// Workspace of the path for many rows: flags, partial records, scales, rows.
+struct ManyLayout {
+  size_t scales, rows, total;
+};
+ManyLayout many_layout(int32_t kv_len, int32_t hkv) {
+  ManyLayout m;
+  m.scales = hsd_host::kKv8FlagBytes + align256(hsd_host::attention_partials_bytes());
+  m.rows = m.scales + align256(size_t(hkv) * ((kv_len + 127) / 128) * 2 * sizeof(hsd::attn::ColumnScale));
+  m.total = m.rows + size_t(2) * hkv * kv_len * hsd::kv8a::HD * 2;
+  return m;
+}
+
+// Rows kernel or many rows.
+bool use_rows(int32_t q_len, int32_t group) { return int64_t(q_len) * group <= 256; }
+
+int many_launch(const hsd_host::Kv8AttnArgs& a, const hsd_plan_t& plan, float scale) {
+  using namespace hsd;
+  const kv8a::Params& p = a.p;
+  int rc = hsd_host::attention_check_tiles(plan, "hsd_verify_attention_kv8");
+  if (rc) return rc;
+  if (256 + hsd_host::attention_flags_bytes() > hsd_host::kKv8FlagBytes || p.hkv > 65535) {
+    hsd_host::set_error("hsd_verify_attention_kv8: %d KV heads exceed the launch's range", p.hkv);
+    return HSD_ERR_TOO_LARGE;
+  }
+  const ManyLayout m = many_layout(p.kv_len, p.hkv);
+  char* ws = static_cast<char*>(a.workspace);
+  kv8a::ExpandParams e;
+  e.x8[0] = a.k8;
+  e.x8[1] = a.v8;
+  e.head_stride8[0] = a.k8_head_stride;
+  e.head_stride8[1] = a.v8_head_stride;
+  e.scale[0] = p.k_scale;
+  e.scale[1] = p.v_scale;
+  e.scale_stride = p.scale_stride;
+  e.tail[0] = static_cast<const __nv_bfloat16*>(a.k_tail);
+  e.tail[1] = static_cast<const __nv_bfloat16*>(a.v_tail);
+  e.row_stride[0] = a.kt_row_stride;
+  e.row_stride[1] = a.vt_row_stride;
+  e.head_stride[0] = a.kt_head_stride;
+  e.head_stride[1] = a.vt_head_stride;
+  e.tile_class = plan.tile_class;
+  e.mask_words = plan.mask_words;
+  e.dst = reinterpret_cast<__nv_bfloat16*>(ws + m.rows);
+  e.col_scale = reinterpret_cast<attn::ColumnScale*>(ws + m.scales);
+  e.kv_len = p.kv_len;
+  e.hkv = p.hkv;
+  e.n_kv64 = p.n_kv64;
+  e.n_qtiles = plan.n_qtiles;
+  e.sealed = p.sealed;
+  e.tail_row0 = p.tail_row0;
+  e.scale_log2 = p.scale_log2;
+  rc = hsd_host::launch_pdl(kv8a::expand_kernel,
+                            dim3(unsigned(p.n_kv64), unsigned(p.hkv), 2),
+                            dim3(kv8a::kExpandThreads), 0, a.stream, "expand_kernel launch", 0, e);
+  if (rc) return rc;
+  hsd_host::AttentionArgs v;
+  v.q = p.q;
+  v.q_row_stride = p.q_row_stride;
+  v.q_head_stride = p.q_head_stride;
+  v.k = e.dst;
+  v.v = e.dst + size_t(p.hkv) * p.kv_len * kv8a::HD;
+  v.k_row_stride = v.v_row_stride = kv8a::HD;
+  v.k_head_stride = v.v_head_stride = int64_t(p.kv_len) * kv8a::HD;
+  v.out = p.out;
+  v.lse = p.lse;
+  v.q_len = p.q_len;
+  v.kv_len = p.kv_len;
+  v.num_q_heads = p.hq;
+  v.num_kv_heads = p.hkv;
+  v.scale = scale;
+  v.plan = &plan;
+  v.sync = reinterpret_cast<uint32_t*>(ws);
+  v.flags = reinterpret_cast<uint32_t*>(ws + 256);
+  v.partials = ws + hsd_host::kKv8FlagBytes;
+  v.status = p.status;
+  v.stream = reinterpret_cast<hsd_stream_t>(a.stream);
+  v.col_scale = e.col_scale;
+  return hsd_host::attention_launch(v);
+}
 
 bool strides_ok(const void* p, int64_t rs, int64_t hs) {
   return p && (reinterpret_cast<uintptr_t>(p) & 15) == 0 && rs > 0 && hs > 0 && (rs % 8) == 0 &&
@@ -16,7 +215,9 @@ extern "C" size_t hsd_kv8_attention_workspace_bytes(int32_t q_len, int32_t kv_le
   if (q_len <= 0 || kv_len <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 ||
       num_q_heads % num_kv_heads)
     return 0;
-  return hsd_host::kv8_rows_workspace_bytes(q_len, kv_len, num_q_heads, num_kv_heads);
+  if (use_rows(q_len, num_q_heads / num_kv_heads))
+    return hsd_host::kv8_rows_workspace_bytes(q_len, kv_len, num_q_heads, num_kv_heads);
+  return many_layout(kv_len, num_kv_heads).total;
 }
 
 extern "C" int hsd_verify_attention_kv8(
@@ -102,5 +303,5 @@ extern "C" int hsd_verify_attention_kv8(
   a.vt_head_stride = vt_head_stride;
   a.workspace = workspace;
   a.stream = reinterpret_cast<cudaStream_t>(stream);
-  return hsd_host::kv8_rows_launch(a);
+  return use_rows(q_len, p.group) ? hsd_host::kv8_rows_launch(a) : many_launch(a, *plan, scale);
 }

@@ -45,9 +45,19 @@
 // pieces from the previous one (the next head pair or tile) after one binary
 // search for the first.  The MMA thread releases Q after the piece's last S,
 // so the next piece's Q loads under the last block's softmax and PV.
+//
+// kScaled (the attention over the 8-bit cache, kv8_attn.cu): every 64 columns
+// have a K scale, which multiplies their scores, and a V scale, which enters
+// the exponent as its logarithm and is divided out of their part of the row
+// sum, so P carries it at no cost per element.  The partial records hold fp16
+// with a power of two per row there (2^-12 of the row's largest value): bf16
+// records add as much error as P's own rounding.
 #include <atomic>
 
 #include "common.cuh"
+#include "verify_attn.cuh"
+
+#include <cuda_fp16.h>
 
 namespace hsd {
 namespace attn {
@@ -57,6 +67,7 @@ constexpr int BN = 128;  // KV columns per block
 constexpr int HD = 128;  // head dim
 constexpr int NSLOT = 2;
 constexpr int NSTAGE = 3;
+constexpr int NSCALE = 4;
 constexpr int TILE_BYTES = BN * HD * 2;  // 32 KB: a 128x128 bf16 tile
 constexpr int SUB_BYTES = 128 * 128;     // one 64-column swizzled sub-tile of 128 rows
 constexpr int kThreads = 384;  // 3 warpgroups: softmax slot 0, slot 1, producer + MMA
@@ -75,12 +86,18 @@ constexpr int kMaxTiles = 1024;  // query tiles per launch (q_len <= 131072)
 // CTA's first piece when that piece continues an item begun by an earlier CTA,
 // as [16 chunks][128 rows] of 16-byte vectors (a warp reads or writes 512
 // contiguous bytes per access), then (m, l) per row in fp32.  Units of 4 bytes.
+// kScaled: fp16, and the rows' powers of two [G][NSLOT][128] follow all records.
 constexpr int kRecWords = 128 * 64 + 128 * 2;
 
 struct __align__(1024) Smem {
   uint8_t q[NSLOT][TILE_BYTES];
   uint8_t pb[NSLOT][TILE_BYTES];  // P of the current block per slot (MMA A operand)
   uint8_t kv[NSTAGE][TILE_BYTES];
+  // kScaled: the scales of a block's halves, four blocks in turn, copied with
+  // its K tile.  Block n + 3's K tile is loaded after PV(n), hence after the
+  // softmax of block n.
+  ColumnScale scales[NSCALE][2];
+  uint64_t bar_scales[NSCALE];
   uint64_t bar_q;
   uint64_t bar_q_free;
   uint64_t bar_full[NSTAGE];
@@ -120,7 +137,14 @@ struct Params {
   int n_qtiles, n_kv64, n_kv128;
   float scale_log2;
   int split;  // 1: stream-K over gridDim.x CTAs; 0: one item per CTA
+  const ColumnScale* col_scale;  // [hkv][2 n_kv128], kScaled
 };
+
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
 
 // A piece: blocks [b0, b1) of one item (query tile x head pair).
 struct Piece {
@@ -191,6 +215,15 @@ __device__ __forceinline__ int range_start(int k, int total, int g) {
 constexpr uint32_t kIdescS = idesc_bf16_f32(BM, BN, false, false);  // Q K^T: both K-major
 constexpr uint32_t kIdescO = idesc_bf16_f32(BM, HD, false, true);   // P V: V is MN-major
 
+__device__ __forceinline__ float sum8(const uint64_t (&s)[4]) {
+  float s0, s1, s2, s3, s4, s5, s6, s7;
+  f2_unpack(s[0], s0, s1);
+  f2_unpack(s[1], s2, s3);
+  f2_unpack(s[2], s4, s5);
+  f2_unpack(s[3], s6, s7);
+  return ((s0 + s1) + (s2 + s3)) + ((s4 + s5) + (s6 + s7));
+}
+
 // S = Q K^T for one 128x128 block: 8 MMAs of K = 16.  Descriptors advance
 // inside a 128-byte swizzle atom by adding the byte offset >> 4 to the start
 // address field (two 64-column sub-tiles of 16 KB each).
@@ -218,6 +251,7 @@ __device__ __forceinline__ void issue_pv(uint32_t d_tmem, uint32_t p_smem, uint3
   }
 }
 
+template <bool kScaled>
 __global__ void __launch_bounds__(kThreads, 1)
     verify_attn_kernel(const __grid_constant__ CUtensorMap tm_q,
                        const __grid_constant__ CUtensorMap tm_k,
@@ -238,6 +272,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&sm.bar_full[i], 1);
       mbar_init(&sm.bar_empty[i], NSLOT);
     }
+    if constexpr (kScaled)
+      for (int i = 0; i < NSCALE; ++i) mbar_init(&sm.bar_scales[i], 1);
     for (int i = 0; i < NSLOT; ++i) {
       mbar_init(&sm.bar_s_full[i], 1);
       mbar_init(&sm.bar_s_free[i], 128);
@@ -298,6 +334,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t phase = 0;
       int issued = 0;  // K/V tiles issued; ring slot i was used ceil((issued - i) / NSTAGE) times
       int pieces = 0;
+      int blocks = 0;  // kScaled: blocks whose scales were copied
       bool ok = true;
       int w = w0;
       Piece pc;
@@ -320,6 +357,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int kb = int(list[j] & 0xFFFFFFu);
           ok = mbar_wait(&sm.bar_empty[stage], phase ^ 1u, abort, p.status, 0x100 + int(is_v));
           if (!ok) break;
+          if constexpr (kScaled) {
+            if (!is_v) {
+              uint64_t* bar = &sm.bar_scales[blocks & (NSCALE - 1)];
+              mbar_arrive_expect_tx(bar, 2 * sizeof(ColumnScale));
+              bulk_load(sm.scales[blocks & (NSCALE - 1)],
+                        p.col_scale + size_t(pc.kvh) * (2 * p.n_kv128) + 2 * kb,
+                        2 * sizeof(ColumnScale), bar);
+              ++blocks;
+            }
+          }
           mbar_arrive_expect_tx(&sm.bar_full[stage], TILE_BYTES);
           const CUtensorMap* tm = is_v ? &tm_v : &tm_k;
           for (int d = 0; d < 2; ++d)
@@ -342,6 +389,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (pieces > 0)
         mbar_wait(&sm.bar_q, uint32_t(pieces - 1) & 1u, abort, p.status, 0x120, false);
+      if constexpr (kScaled)
+        for (int i = 0; i < min(blocks, NSCALE); ++i)
+          mbar_wait(&sm.bar_scales[i], uint32_t((blocks - 1 - i) / NSCALE) & 1u, abort, p.status,
+                    0x130 + i, false);
     } else if ((warp == 9 || warp == 11) && lane == 0) {
       // ---------------------------------------------------------- MMA issuers
       // One thread per slot (warp 9: slot 0, warp 11: slot 1), so each slot's
@@ -480,10 +531,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     int hs = 0;  // blocks with both slots active (exponential-phase handshakes)
     bool ok = true;
     bool pub_wait = false;  // the P buffer holds a staged record warp 10 may not have read
+    int nb = 0;  // kScaled: blocks of the CTA before this one
     int w = w0;
     Piece pc;
     while (ok && next_piece(p, w, w1, pc)) {
-      if (s >= pc.nslot) continue;
+      if (s >= pc.nslot) {
+        if constexpr (kScaled) nb += pc.b1 - pc.b0;
+        continue;
+      }
       const int qt = pc.qt;
       const int q = qt * BM + r;
       const int h = pc.h0 + s;
@@ -508,6 +563,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t mw[4] = {uint32_t(wd_next[0]), uint32_t(wd_next[0] >> 32), uint32_t(wd_next[1]),
                           uint32_t(wd_next[1] >> 32)};
         if (j + 1 < pc.b1) e_next = list[j + 1];
+        const ColumnScale* sc = sm.scales[nb & (NSCALE - 1)];
+        if constexpr (kScaled) {
+          ok = __all_sync(0xffffffffu,
+                          mbar_wait(&sm.bar_scales[nb & (NSCALE - 1)], uint32_t(nb / NSCALE) & 1u,
+                                    abort, p.status, 0x302 + s));
+          if (!ok) break;
+          ++nb;
+        }
         ok = __all_sync(0xffffffffu, mbar_wait(&sm.bar_s_full[s], uint32_t(gs) & 1u, abort,
                                                p.status, 0x300 + s));
         if (!ok) break;
@@ -533,19 +596,38 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int i = 0; i < 128; ++i)
             x[i] = ((mw[i >> 5] >> (i & 31)) & 1u) ? x[i] : -INFINITY;
         }
-        // row max: eight independent chains, then a tree
-        float mx8[8];
+        float m_new;
+        if constexpr (kScaled) {
+          // per half: four independent chains, then the half's scale
+          float mx4[2][4];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) mx8[k] = x[k];
+          for (int hf = 0; hf < 2; ++hf) {
 #pragma unroll
-        for (int i = 8; i + 16 <= 128; i += 16)
+            for (int k = 0; k < 4; ++k) mx4[hf][k] = fmaxf(x[64 * hf + k], x[64 * hf + 60 + k]);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) mx8[k] = fmax3(mx8[k], x[i + k], x[i + 8 + k]);
+            for (int i = 4; i + 8 <= 60; i += 8)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) mx8[k] = fmaxf(mx8[k], x[120 + k]);
-        const float mx = fmax3(fmax3(mx8[0], mx8[1], mx8[2]), fmax3(mx8[3], mx8[4], mx8[5]),
-                               fmaxf(mx8[6], mx8[7]));
-        const float m_new = fmaxf(m, mx * p.scale_log2);
+              for (int k = 0; k < 4; ++k)
+                mx4[hf][k] = fmax3(mx4[hf][k], x[64 * hf + i + k], x[64 * hf + i + 4 + k]);
+          }
+          m_new = fmax3(m,
+                        fmaxf(fmax3(mx4[0][0], mx4[0][1], mx4[0][2]), mx4[0][3]) * sc[0].score,
+                        fmaxf(fmax3(mx4[1][0], mx4[1][1], mx4[1][2]), mx4[1][3]) * sc[1].score);
+        } else {
+          // row max: eight independent chains, then a tree
+          float mx8[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) mx8[k] = x[k];
+#pragma unroll
+          for (int i = 8; i + 16 <= 128; i += 16)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) mx8[k] = fmax3(mx8[k], x[i + k], x[i + 8 + k]);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) mx8[k] = fmaxf(mx8[k], x[120 + k]);
+          const float mx = fmax3(fmax3(mx8[0], mx8[1], mx8[2]), fmax3(mx8[3], mx8[4], mx8[5]),
+                                 fmaxf(mx8[6], mx8[7]));
+          m_new = fmaxf(m, mx * p.scale_log2);
+        }
         const bool need = m_new > m + kRescaleLog2;  // also true for m = -inf, m_new finite
         const float alpha = need ? ex2_approx(m - m_new) : 1.f;
         if (need) m = m_new;
@@ -604,12 +686,22 @@ __global__ void __launch_bounds__(kThreads, 1)
         // (two 64-column sub-tiles, 128-byte rows, 16-byte chunk c stored at
         // chunk c ^ (r & 7): the TMA / MMA 128-byte swizzle).  The scale,
         // subtract and row sums run on packed fp32 pairs.
-        const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2);
-        const uint64_t nm2 = f2_pack(nm, nm);
+        uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2);
+        uint64_t nm2 = f2_pack(nm, nm);
+        float half_sum = 0.f;  // kScaled: the first half's row sum
         uint64_t sum2[4] = {0ull, 0ull, 0ull, 0ull};
         const uint32_t prow = smem_u32(sm.pb[s]) + uint32_t(r) * 128u;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
+          if constexpr (kScaled) {
+            sc2 = f2_pack(sc[c].score, sc[c].score);
+            nm2 = f2_pack(nm + sc[c].log2_v, nm + sc[c].log2_v);
+            if (c == 1) {
+              half_sum = sum8(sum2) * sc[0].inv_v;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) sum2[i] = 0ull;
+            }
+          }
 #pragma unroll
           for (int ch = 0; ch < 8; ++ch) {
             uint32_t pk[4];
@@ -631,12 +723,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           mbar_arrive(&sm.bar_mufu[s ^ 1]);
           ++hs;
         }
-        float s0, s1, s2, s3, s4, s5, s6, s7;
-        f2_unpack(sum2[0], s0, s1);
-        f2_unpack(sum2[1], s2, s3);
-        f2_unpack(sum2[2], s4, s5);
-        f2_unpack(sum2[3], s6, s7);
-        l = l * alpha + (((s0 + s1) + (s2 + s3)) + ((s4 + s5) + (s6 + s7))) * kPackBiasInv;
+        if constexpr (kScaled)
+          l = l * alpha + (half_sum + sum8(sum2) * sc[1].inv_v) * kPackBiasInv;
+        else
+          l = l * alpha + sum8(sum2) * kPackBiasInv;
         tmem_wait_st();  // O rescale stores, if any
         tc_fence_before();
         fence_async_shared();  // P stores -> visible to the MMA (async proxy)
@@ -674,6 +764,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t* rec = p.partials + (size_t(blockIdx.x) * NSLOT + s) * kRecWords;
         const float invl = (l > 0.f) ? 1.f / l : 0.f;
         const uint32_t stg = smem_u32(sm.pb[s]) + uint32_t(r) * 16u;
+        if constexpr (kScaled) {
+          // fp16 times the power of two at or below the row's largest |O / l|
+          float top = 0.f;
+#pragma unroll
+          for (int i = 0; i < 128; ++i) top = fmaxf(top, fabsf(o[i]));
+          const uint32_t unit =
+              min(max(__float_as_uint(top * invl) & 0x7f800000u, 27u << 23), 247u << 23);
+          const float f = invl * __uint_as_float((254u << 23) - unit);
+#pragma unroll
+          for (int c = 0; c < 16; ++c)
+            st_shared_v4(stg + uint32_t(c) * 2048u, pack_f16x2(o[8 * c] * f, o[8 * c + 1] * f),
+                         pack_f16x2(o[8 * c + 2] * f, o[8 * c + 3] * f),
+                         pack_f16x2(o[8 * c + 4] * f, o[8 * c + 5] * f),
+                         pack_f16x2(o[8 * c + 6] * f, o[8 * c + 7] * f));
+          p.partials[size_t(G) * NSLOT * kRecWords + (size_t(blockIdx.x) * NSLOT + s) * 128 + r] =
+              unit;
+        } else
 #pragma unroll
         for (int c = 0; c < 16; ++c)
           st_shared_v4(stg + uint32_t(c) * 2048u, pack_bf16x2(o[8 * c] * invl, o[8 * c + 1] * invl),
@@ -706,6 +813,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           int4 v[16];
 #pragma unroll
           for (int c = 0; c < 16; ++c) v[c] = __ldcg(rec4 + c * 128 + r);
+          float unit = 1.f;
+          if constexpr (kScaled)
+            unit = __uint_as_float(__ldcg(p.partials + size_t(G) * NSLOT * kRecWords +
+                                          (size_t(k) * NSLOT + s) * 128 + r));
           const bool use = ml.y > 0.f;
           const float nm = use ? fmaxf(m, ml.x) : m;
           const float a = use ? ex2_approx(m - nm) : 1.f;  // 0 when this row had nothing yet
@@ -716,9 +827,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                                     uint32_t(v[c].w)};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              o[8 * c + 2 * i] = o[8 * c + 2 * i] * a + __uint_as_float(wv[i] << 16) * b;
-              o[8 * c + 2 * i + 1] =
-                  o[8 * c + 2 * i + 1] * a + __uint_as_float(wv[i] & 0xffff0000u) * b;
+              if constexpr (kScaled) {
+                const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&wv[i]));
+                o[8 * c + 2 * i] = o[8 * c + 2 * i] * a + t.x * (b * unit);
+                o[8 * c + 2 * i + 1] = o[8 * c + 2 * i + 1] * a + t.y * (b * unit);
+              } else {
+                o[8 * c + 2 * i] = o[8 * c + 2 * i] * a + __uint_as_float(wv[i] << 16) * b;
+                o[8 * c + 2 * i + 1] =
+                    o[8 * c + 2 * i + 1] * a + __uint_as_float(wv[i] & 0xffff0000u) * b;
+              }
             }
           }
           l = l * a + b;
@@ -853,14 +970,11 @@ int sm_count() {
 // [G][NSLOT][4], then {generation, CTAs finished}.  G = SMs of the device.
 struct WsLayout {
   size_t partials, flags, sync, total;
-  int items, grid;
+  int grid;
 };
 
-WsLayout ws_layout(int32_t q_len, int32_t hq, int32_t hkv) {
+WsLayout ws_layout() {
   WsLayout L{};
-  const int n_qtiles = (q_len + attn::BM - 1) / attn::BM;
-  const int group = hq / hkv, pairs = (group + 1) / 2;
-  L.items = n_qtiles * hkv * pairs;
   L.grid = sm_count();
   L.partials = 0;
   L.flags = size_t(L.grid) * attn::NSLOT * attn::kRecWords * sizeof(uint32_t);
@@ -873,13 +987,19 @@ constexpr int kMaxDevices = 64;
 // Per-device "attribute set" flags, atomic: host threads driving different
 // devices or streams may reach them at once (setting the attribute twice is
 // harmless).
-std::atomic<bool> g_attr_set[kMaxDevices];
+std::atomic<bool> g_attr_set[2][kMaxDevices];  // [kScaled][device]
 
 }  // namespace
 
 namespace hsd_host {
-size_t attention_flags_offset(int32_t q_len, int32_t num_q_heads, int32_t num_kv_heads) {
-  return ws_layout(q_len, num_q_heads, num_kv_heads).flags;
+size_t attention_partials_bytes() {
+  return size_t(sm_count()) * attn::NSLOT * (attn::kRecWords + 128) * sizeof(uint32_t);
+}
+size_t attention_flags_bytes() {
+  return size_t(sm_count()) * attn::NSLOT * 4 * sizeof(uint32_t);
+}
+size_t attention_flags_offset(int32_t, int32_t, int32_t) {
+  return ws_layout().flags;
 }
 }  // namespace hsd_host
 
@@ -887,8 +1007,90 @@ extern "C" size_t hsd_attention_workspace_bytes(int32_t q_len, int32_t num_q_hea
                                                 int32_t num_kv_heads) {
   if (q_len <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads)
     return 0;
-  return ws_layout(q_len, num_q_heads, num_kv_heads).total;
+  return ws_layout().total;
 }
+
+namespace hsd_host {
+
+int attention_check_tiles(const hsd_plan_t& plan, const char* what) {
+  if (plan.n_qtiles <= attn::kMaxTiles) return HSD_OK;
+  set_error("%s: q_len %d exceeds %d query tiles", what, plan.q_len, attn::kMaxTiles);
+  return HSD_ERR_TOO_LARGE;
+}
+
+int attention_launch(const AttentionArgs& a) {
+  const bool scaled = a.col_scale != nullptr;
+  CUtensorMap tq, tk, tv;
+  int rc = make_map(&tq, a.q, a.q_len, a.num_q_heads, a.q_row_stride, a.q_head_stride, "q");
+  if (!rc) rc = make_map(&tk, a.k, a.kv_len, a.num_kv_heads, a.k_row_stride, a.k_head_stride, "k");
+  if (!rc) rc = make_map(&tv, a.v, a.kv_len, a.num_kv_heads, a.v_row_stride, a.v_head_stride, "v");
+  CUtensorMap to;
+  if (!rc)
+    rc = make_map(&to, a.out, a.q_len, a.num_q_heads, int64_t(a.num_q_heads) * attn::HD, attn::HD,
+                  "out");
+  if (rc) return rc;
+  attn::Params p;
+  p.out = static_cast<__nv_bfloat16*>(a.out);
+  p.lse = a.lse;
+  p.blk_list = a.plan->blk_list;
+  p.blk_count = a.plan->blk_count;
+  p.mask_words = a.plan->mask_words;
+  p.tile_order = a.plan->tile_order;
+  p.blk_prefix = a.plan->blk_prefix;
+  p.status = a.status;
+  p.q_len = a.q_len;
+  p.kv_len = a.kv_len;
+  p.hq = a.num_q_heads;
+  p.hkv = a.num_kv_heads;
+  p.group = a.num_q_heads / a.num_kv_heads;
+  p.pairs = (p.group + 1) / 2;
+  p.n_qtiles = a.plan->n_qtiles;
+  p.n_kv64 = a.plan->n_kv64;
+  p.n_kv128 = a.plan->n_kv128;
+  p.scale_log2 = a.scale * 1.4426950408889634f;
+  const bool split = a.partials != nullptr;
+  p.split = split ? 1 : 0;
+  p.partials = static_cast<uint32_t*>(a.partials);
+  p.flags = a.flags;
+  p.sync = a.sync;
+  p.col_scale = a.col_scale;
+  const size_t smem = sizeof(attn::Smem) + 1024;
+  int dev = 0;
+  rc = hsd_host::cuda_check(cudaGetDevice(&dev), "cudaGetDevice");
+  if (rc) return rc;
+  if (dev < 0 || dev >= kMaxDevices) {
+    hsd_host::set_error("hsd_verify_attention: device ordinal %d >= %d", dev, kMaxDevices);
+    return HSD_ERR_UNSUPPORTED;
+  }
+  const auto kernel = scaled ? attn::verify_attn_kernel<true> : attn::verify_attn_kernel<false>;
+  if (!g_attr_set[scaled][dev].load(std::memory_order_acquire)) {
+    rc = hsd_host::cuda_check(
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)),
+        "cudaFuncSetAttribute(verify_attn_kernel)");
+    if (rc) return rc;
+    g_attr_set[scaled][dev].store(true, std::memory_order_release);
+  }
+  // stream-K: one CTA per SM sharing the total work evenly; otherwise one CTA
+  // per (query tile, head pair) item.
+  const int grid = split ? sm_count() : p.n_qtiles * p.hkv * p.pairs;
+  // Programmatic dependent launch: the CTAs may start their setup while the
+  // previous kernel on the stream finishes (griddepcontrol.wait in the
+  // kernel holds every read of global memory until it has completed).
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(grid));
+  cfg.blockDim = dim3(attn::kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = reinterpret_cast<cudaStream_t>(a.stream);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return hsd_host::cuda_check(cudaLaunchKernelEx(&cfg, kernel, tq, tk, tv, to, p),
+                              "verify_attn_kernel launch");
+}
+
+}  // namespace hsd_host
 
 extern "C" int hsd_verify_attention(const void* q, int64_t q_row_stride, int64_t q_head_stride,
                                     const void* k, int64_t k_row_stride, int64_t k_head_stride,
@@ -913,82 +1115,39 @@ extern "C" int hsd_verify_attention(const void* q, int64_t q_row_stride, int64_t
         plan ? plan->kv_len : -1);
     return HSD_ERR_INVALID_ARG;
   }
-  if (plan->n_qtiles > attn::kMaxTiles) {
-    hsd_host::set_error("hsd_verify_attention: q_len %d exceeds %d query tiles", q_len,
-                        attn::kMaxTiles);
-    return HSD_ERR_TOO_LARGE;
-  }
-  const WsLayout W = ws_layout(q_len, num_q_heads, num_kv_heads);
+  int rc = hsd_host::attention_check_tiles(*plan, "hsd_verify_attention");
+  if (rc) return rc;
+  const WsLayout W = ws_layout();
   const bool split = workspace != nullptr;
   if (split && ((reinterpret_cast<uintptr_t>(workspace) & 255) || workspace_bytes < W.total)) {
     hsd_host::set_error("hsd_verify_attention: workspace %zu bytes (need %zu, 256-byte aligned)",
                         workspace_bytes, W.total);
     return HSD_ERR_INVALID_ARG;
   }
-  CUtensorMap tq, tk, tv;
-  int rc = make_map(&tq, q, q_len, num_q_heads, q_row_stride, q_head_stride, "q");
-  if (!rc) rc = make_map(&tk, k, kv_len, num_kv_heads, k_row_stride, k_head_stride, "k");
-  if (!rc) rc = make_map(&tv, v, kv_len, num_kv_heads, v_row_stride, v_head_stride, "v");
-  CUtensorMap to;
-  if (!rc)
-    rc = make_map(&to, out, q_len, num_q_heads, int64_t(num_q_heads) * attn::HD, attn::HD, "out");
-  if (rc) return rc;
-  attn::Params p;
-  p.out = static_cast<__nv_bfloat16*>(out);
-  p.lse = lse;
-  p.blk_list = plan->blk_list;
-  p.blk_count = plan->blk_count;
-  p.mask_words = plan->mask_words;
-  p.tile_order = plan->tile_order;
-  p.blk_prefix = plan->blk_prefix;
-  p.status = status;
-  p.q_len = q_len;
-  p.kv_len = kv_len;
-  p.hq = num_q_heads;
-  p.hkv = num_kv_heads;
-  p.group = num_q_heads / num_kv_heads;
-  p.pairs = (p.group + 1) / 2;
-  p.n_qtiles = plan->n_qtiles;
-  p.n_kv64 = plan->n_kv64;
-  p.n_kv128 = plan->n_kv128;
-  p.scale_log2 = scale * 1.4426950408889634f;
-  p.split = split ? 1 : 0;
+  hsd_host::AttentionArgs a;
+  a.q = q;
+  a.q_row_stride = q_row_stride;
+  a.q_head_stride = q_head_stride;
+  a.k = k;
+  a.k_row_stride = k_row_stride;
+  a.k_head_stride = k_head_stride;
+  a.v = v;
+  a.v_row_stride = v_row_stride;
+  a.v_head_stride = v_head_stride;
+  a.out = out;
+  a.lse = lse;
+  a.q_len = q_len;
+  a.kv_len = kv_len;
+  a.num_q_heads = num_q_heads;
+  a.num_kv_heads = num_kv_heads;
+  a.scale = scale;
+  a.plan = plan;
   char* ws = static_cast<char*>(workspace);
-  p.partials = split ? reinterpret_cast<uint32_t*>(ws + W.partials) : nullptr;
-  p.flags = split ? reinterpret_cast<uint32_t*>(ws + W.flags) : nullptr;
-  p.sync = split ? reinterpret_cast<uint32_t*>(ws + W.sync) : nullptr;
-  const size_t smem = sizeof(attn::Smem) + 1024;
-  int dev = 0;
-  rc = hsd_host::cuda_check(cudaGetDevice(&dev), "cudaGetDevice");
-  if (rc) return rc;
-  if (dev < 0 || dev >= kMaxDevices) {
-    hsd_host::set_error("hsd_verify_attention: device ordinal %d >= %d", dev, kMaxDevices);
-    return HSD_ERR_UNSUPPORTED;
-  }
-  if (!g_attr_set[dev].load(std::memory_order_acquire)) {
-    rc = hsd_host::cuda_check(
-        cudaFuncSetAttribute(attn::verify_attn_kernel,
-                             cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)),
-        "cudaFuncSetAttribute(verify_attn_kernel)");
-    if (rc) return rc;
-    g_attr_set[dev].store(true, std::memory_order_release);
-  }
-  // stream-K: one CTA per SM sharing the total work evenly; otherwise one CTA
-  // per (query tile, head pair) item.
-  const int grid = split ? W.grid : W.items;
-  // Programmatic dependent launch: the CTAs may start their setup while the
-  // previous kernel on the stream finishes (griddepcontrol.wait in the
-  // kernel holds every read of global memory until it has completed).
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(grid));
-  cfg.blockDim = dim3(attn::kThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = reinterpret_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return hsd_host::cuda_check(cudaLaunchKernelEx(&cfg, attn::verify_attn_kernel, tq, tk, tv, to, p),
-                              "verify_attn_kernel launch");
+  a.partials = split ? ws + W.partials : nullptr;
+  a.flags = split ? reinterpret_cast<uint32_t*>(ws + W.flags) : nullptr;
+  a.sync = split ? reinterpret_cast<uint32_t*>(ws + W.sync) : nullptr;
+  a.status = status;
+  a.stream = stream;
+  a.col_scale = nullptr;
+  return hsd_host::attention_launch(a);
 }

@@ -394,8 +394,8 @@ int hsd_kv8_unseal(const int8_t *data, int64_t plane_stride, const float *scale,
  * v_scale: one per 64 rows, heads scale_head_stride apart.  Either side may
  * be empty, its pointers then NULL.  The mask, out, lse and the strides of q
  * and the tails are those of hsd_verify_attention; fully masked rows give 0
- * and -inf, and what stands in a bf16 column that no query row of the tile
- * sees does not matter.  P is rounded to bf16, everything else is fp32.
+ * and -inf, and what stands in a bf16 column that no query row sees does not
+ * matter.  P is rounded to bf16, everything else is fp32.
  * workspace: hsd_kv8_attention_workspace_bytes, 256-byte aligned, its first
  * 64 KB zero-filled before the first use; each call leaves it ready for the
  * next (after an error status, zero them again), and calls sharing one must
