@@ -9,6 +9,7 @@ entry point returns a non-zero status.  Structures mirror
 from __future__ import annotations
 
 import ctypes as C
+import importlib.util
 import os
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libhsd_b200.so")
@@ -151,6 +152,28 @@ def load():
         fn.argtypes = args
     _lib = lib
     return lib
+
+
+_ops = None
+
+
+def ops():
+    """The compiled Python binding ``_ops.so`` (csrc/ops.cpp), loaded once."""
+    global _ops
+    if _ops is None:
+        load()
+        import torch  # noqa: F401  (the binding's libraries)
+        path = os.path.join(os.path.dirname(LIB_PATH), "_ops.so")
+        if not os.path.exists(path):
+            raise HSDNativeError(f"{path} is missing: build it with `python -m hsd_b200.build`")
+        try:
+            spec = importlib.util.spec_from_file_location("hsd_b200._ops", path)
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+        except ImportError as e:
+            raise HSDNativeError(f"cannot load {path}: {e}") from e
+        _ops = module
+    return _ops
 
 
 def check(rc: int, what: str):

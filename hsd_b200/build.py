@@ -5,9 +5,11 @@
 Compiles every ``hsd_b200/csrc/*.cu`` with nvcc
 (``-gencode arch=compute_100a,code=sm_100a -lineinfo -O3``) and links them
 into one shared library with the CUDA runtime linked statically, so the
-library loads next to PyTorch's own runtime without version coupling.  The
-build is incremental: nothing is recompiled when the library is newer than
-every source and header.
+library loads next to PyTorch's own runtime without version coupling.  Then
+compiles ``csrc/ops.cpp``, the Python binding of the entry points whose calls
+have to be cheap on the host (``hsd_b200/_ops.so``; it links PyTorch and the
+library).  The build is incremental: nothing is recompiled when the outputs
+are newer than every source and header.
 """
 from __future__ import annotations
 
@@ -16,12 +18,14 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 LIB = os.path.join(PKG, "libhsd_b200.so")
+OPS = os.path.join(PKG, "_ops.so")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -41,16 +45,57 @@ def _deps():
         glob.glob(os.path.join(INCLUDE, "*.h"))
 
 
-def up_to_date():
-    if not os.path.exists(LIB):
+def _newer(out, deps):
+    if not os.path.exists(out):
         return False
-    t = os.path.getmtime(LIB)
-    return all(os.path.getmtime(p) <= t for p in _deps())
+    t = os.path.getmtime(out)
+    return all(os.path.getmtime(p) <= t for p in deps)
+
+
+def up_to_date():
+    return _newer(LIB, _deps()) and _newer(OPS, _ops_deps())
+
+
+def _ops_deps():
+    return [os.path.join(CSRC, "ops.cpp")] + glob.glob(os.path.join(INCLUDE, "*.h"))
+
+
+def _ops_command(out):
+    """The host compiler's command for the Python binding; its symbols of the
+    library resolve in ``libhsd_b200.so`` beside it, PyTorch's in the libraries
+    that ``import torch`` has loaded."""
+    import torch
+    cxx = os.environ.get("CXX") or shutil.which("g++")
+    if not cxx:
+        raise RuntimeError("g++ not found; the Python binding needs a host compiler")
+    cuda = os.path.join(os.path.dirname(os.path.dirname(nvcc_path())), "include")
+    home = os.path.dirname(torch.__file__)
+    inc = [INCLUDE, cuda, sysconfig.get_paths()["include"], os.path.join(home, "include"),
+           os.path.join(home, "include", "torch", "csrc", "api", "include")]
+    lib = os.path.join(home, "lib")
+    return [cxx, "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            os.path.join(CSRC, "ops.cpp"), "-o", out] + ["-I" + d for d in inc] + \
+        ["-L" + PKG, "-l:libhsd_b200.so", "-Wl,-rpath,$ORIGIN", "-L" + lib, "-ltorch_python",
+         "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_cuda"]
 
 
 def build(verbose=False, force=False, jobs=None):
-    if not force and up_to_date():
-        return LIB
+    if force or not _newer(LIB, _deps()):
+        _build_library(verbose)
+    if force or not _newer(OPS, _ops_deps()):
+        tmp = OPS + ".tmp"
+        r = subprocess.run(_ops_command(tmp), stdout=subprocess.PIPE, stderr=subprocess.STDOUT,
+                           text=True)
+        if verbose or r.returncode:
+            sys.stderr.write(r.stdout)
+        if r.returncode:
+            raise RuntimeError("the Python binding (csrc/ops.cpp) failed to build")
+        os.replace(tmp, OPS)
+    return LIB
+
+
+def _build_library(verbose):
     nvcc = nvcc_path()
     objdir = os.path.join(PKG, "_build")
     os.makedirs(objdir, exist_ok=True)
@@ -83,7 +128,6 @@ def build(verbose=False, force=False, jobs=None):
         sys.stderr.write(r.stdout)
         raise RuntimeError("nvcc link failed building hsd_b200")
     os.replace(tmp, LIB)
-    return LIB
 
 
 if __name__ == "__main__":

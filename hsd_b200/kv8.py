@@ -17,14 +17,11 @@ The reference has no such cache (its ``DynamicCache`` holds bf16, D:356-359).
 """
 from __future__ import annotations
 
-import ctypes as C
-import math
 from typing import NamedTuple
 
 import torch
 
 from . import _native as N
-from .attention import _as_heads
 from .plan import TilePlan
 
 BLOCK = 64  # rows that share a scale
@@ -61,13 +58,6 @@ class Kv8Cache:
         self.status = torch.zeros(1, dtype=torch.int32, device=device)
         self.sealed = 0
 
-    def _planes(self, planes, what):
-        n = self.layers * 2 * self.num_kv_heads
-        if planes.dtype != torch.int64 or planes.numel() != n or not planes.is_contiguous():
-            raise ValueError(f"{what}: {n} plane addresses (int64) are needed")
-        if planes.device != self.data.device:
-            raise ValueError(f"{what}: the planes' addresses must be on {self.data.device}")
-
     def seal(self, planes, n_rows, src_row0=None):
         """Seal the next ``n_rows`` rows (a multiple of 64) of every plane,
         read from row ``src_row0`` on (default: the row of the same number).
@@ -77,31 +67,16 @@ class Kv8Cache:
         Infinities saturate and NaN become 0; either is reported
         (:meth:`raise_on_device_error`).
         """
-        self._planes(planes, "seal")
-        row0 = self.sealed if src_row0 is None else int(src_row0)
-        if n_rows < 0 or n_rows % BLOCK or self.sealed + n_rows > self.capacity or row0 < 0:
-            raise ValueError(f"seal: {n_rows} rows from {row0} (a multiple of {BLOCK}) after "
-                             f"{self.sealed} of {self.capacity}")
-        with torch.cuda.device(self.data.device):
-            N.check(N.load().hsd_kv8_seal(
-                N.ptr(planes), planes.numel(), row0, N.ptr(self.data), self.data.stride(2),
-                N.ptr(self.scale), self.scale.stride(2), self.sealed // BLOCK, n_rows // BLOCK,
-                N.ptr(self.status), N.stream_handle()), "hsd_kv8_seal")
+        N.ops().kv8_seal(planes, self.sealed if src_row0 is None else src_row0, self.data,
+                         self.scale, self.sealed, n_rows, self.status)
         self.sealed += n_rows
 
     def unseal(self, planes, row0, n_rows, dst_row0=None):
         """Rows ``[row0, row0 + n_rows)`` of every plane back as bf16, to rows
         ``dst_row0`` on (default: the same rows) of ``planes``; any row range
         of the sealed ones."""
-        self._planes(planes, "unseal")
-        dst = row0 if dst_row0 is None else int(dst_row0)
-        if row0 < 0 or n_rows < 0 or row0 + n_rows > self.sealed or dst < 0:
-            raise ValueError(f"unseal: rows {row0}..{row0 + n_rows} of {self.sealed} to {dst}")
-        with torch.cuda.device(self.data.device):
-            N.check(N.load().hsd_kv8_unseal(
-                N.ptr(self.data), self.data.stride(2), N.ptr(self.scale), self.scale.stride(2),
-                planes.numel(), row0, n_rows, N.ptr(planes), dst, N.stream_handle()),
-                "hsd_kv8_unseal")
+        N.ops().kv8_unseal(self.data, self.scale, self.sealed, planes, row0, n_rows,
+                           row0 if dst_row0 is None else dst_row0)
 
     def reset(self, sealed=0):
         """Keep only the first ``sealed`` rows (a multiple of 64)."""
@@ -119,49 +94,6 @@ class Kv8Cache:
         if code:
             raise N.HSDError(f"device status 0x{code:x} while sealing (0x{N.HSD_DEV_BAD_VALUE:x}: "
                              "an infinity or NaN among the rows)")
-
-
-_workspaces = {}
-_FLAG_BYTES = 65536  # leading part of the workspace that starts as zeros
-
-
-def _workspace(need, device):
-    """Scratch of (device, current stream), grown to fit; its flags are zeroed
-    once and every call leaves them ready for the next.  A call that is being
-    captured into a graph gets scratch of its own, zeroed by the graph, so
-    graphs that share no stream share no scratch either (replays of one graph
-    never overlap)."""
-    if torch.cuda.is_current_stream_capturing():
-        buf = torch.empty(need + 256, dtype=torch.uint8, device=device)
-        buf[:_FLAG_BYTES + 256].zero_()
-        return buf
-    key = (device.index, int(torch.cuda.current_stream(device).cuda_stream))
-    buf = _workspaces.get(key)
-    if buf is None or buf.numel() < need + 256:
-        buf = torch.zeros(max(need, 1 << 20) + 256, dtype=torch.uint8, device=device)
-        _workspaces[key] = buf
-    return buf
-
-
-def _layer_tensors(layer, sealed, hkv, dev):
-    """Addresses and strides of a layer's sealed rows, checked."""
-    k8, v8, ks, vs = layer
-    for t, name in ((k8, "k"), (v8, "v")):
-        if t.dtype != torch.int8 or t.dim() != 3 or t.shape[0] != hkv or t.shape[2] != 128 \
-                or t.shape[1] < sealed or t.stride(2) != 1 or t.stride(1) != 128:
-            raise ValueError(f"layer.{name}: int8 [{hkv}, >= {sealed}, 128] with contiguous rows")
-    for t, name in ((ks, "k_scale"), (vs, "v_scale")):
-        if t.dtype != torch.float32 or t.dim() != 2 or t.shape[0] != hkv \
-                or t.shape[1] < sealed // BLOCK or t.stride(1) != 1:
-            raise ValueError(f"layer.{name}: float32 [{hkv}, >= {sealed // BLOCK}]")
-    if hkv > 1 and ks.stride(0) != vs.stride(0):
-        raise ValueError("layer: k_scale and v_scale must share a head stride")
-    if any(t.device != dev for t in layer):
-        raise ValueError(f"layer: tensors must be on {dev}")
-    # the head stride of a single head is never used
-    h8 = [t.stride(0) if hkv > 1 else t.shape[1] * 128 for t in (k8, v8)]
-    return (N.ptr(k8), h8[0], N.ptr(v8), h8[1], N.ptr(ks), N.ptr(vs),
-            ks.stride(0) if hkv > 1 else sealed // BLOCK)
 
 
 def verify_attention_kv8(q, layer, sealed, k, v, plan: TilePlan, scale=None, tail_row0=0,
@@ -183,64 +115,5 @@ def verify_attention_kv8(q, layer, sealed, k, v, plan: TilePlan, scale=None, tai
     :func:`verify_attention`); scores, sums and the joined partial rows are
     fp32.
     """
-    q = _as_heads(q, "query")
-    hq, q_len, d = q.shape
-    dev, kv_len = q.device, plan.kv_len
-    if d != 128:
-        raise ValueError(f"query: head_dim {d} (128 only)")
-    if not q.is_cuda or torch.device(plan.workspace.device) != dev:
-        raise ValueError("query and plan must be on the same CUDA device")
-    if plan.q_len != q_len:
-        raise ValueError(f"plan is for {plan.q_len} rows, query has {q_len}")
-    sealed, tail_row0 = int(sealed), int(tail_row0)
-    if sealed < 0 or sealed % BLOCK or sealed > kv_len or not 0 <= tail_row0 <= sealed:
-        raise ValueError(f"sealed={sealed} must be a multiple of {BLOCK} in [0, {kv_len}] and "
-                         f"tail_row0={tail_row0} in [0, sealed]")
-    if sealed < kv_len:
-        if k is None or v is None:
-            raise ValueError(f"columns {sealed}..{kv_len} need the bf16 tail")
-        k, v = _as_heads(k, "key"), _as_heads(v, "value")
-        hkv = k.shape[0]
-        if v.shape[0] != hkv or k.shape[2] != 128 or v.shape[2] != 128 \
-                or min(k.shape[1], v.shape[1]) < kv_len - tail_row0:
-            raise ValueError(f"tail: key {tuple(k.shape)} and value {tuple(v.shape)} must be "
-                             f"[Hkv, >= {kv_len - tail_row0}, 128]")
-        if k.device != dev or v.device != dev:
-            raise ValueError(f"tail: tensors must be on {dev}")
-        # the head stride of a single head is never used
-        tail = []
-        for t in (k, v):
-            tail += [N.ptr(t), t.stride(1), t.stride(0) if hkv > 1 else t.shape[1] * t.stride(1)]
-    else:
-        hkv = layer.k.shape[0]
-        tail = [None, 0, 0, None, 0, 0]
-    if hq % hkv:
-        raise ValueError(f"{hq} query heads over {hkv} KV heads")
-    if sealed:
-        if layer is None:
-            raise ValueError("sealed columns need the layer's tensors")
-        sealed_args = _layer_tensors(layer, sealed, hkv, dev)
-    else:
-        sealed_args = (None, 0, None, 0, None, None, 0)
-    if scale is None:
-        scale = 1.0 / math.sqrt(d)
-    if out is None:
-        out = torch.empty((q_len, hq, d), dtype=torch.bfloat16, device=dev)
-    if need_lse and lse is None:
-        lse = torch.empty((hq, q_len), dtype=torch.float32, device=dev)
-    for t, dt, shape in ((out, torch.bfloat16, (q_len, hq, d)),
-                         (lse if need_lse else None, torch.float32, (hq, q_len))):
-        if t is not None and (t.dtype != dt or tuple(t.shape) != shape or not t.is_contiguous()
-                              or t.device != dev):
-            raise ValueError(f"output must be contiguous {dt} {shape} on {dev}")
-    lib = N.load()
-    with torch.cuda.device(dev):
-        need = lib.hsd_kv8_attention_workspace_bytes(q_len, kv_len, hq, hkv)
-        ws = _workspace(need, dev)
-        N.check(lib.hsd_verify_attention_kv8(
-            N.ptr(q), q.stride(1), q.stride(0) if hq > 1 else q_len * q.stride(1), *sealed_args[:7],
-            sealed, *tail, tail_row0, N.ptr(out), N.ptr(lse) if need_lse else None, q_len, kv_len,
-            hq, hkv, d, float(scale), C.byref(plan.struct),
-            C.c_void_p((ws.data_ptr() + 255) & ~255), need, N.ptr(plan.status),
-            N.stream_handle()), "hsd_verify_attention_kv8")
-    return out, lse if need_lse else None
+    return N.ops().verify_attention_kv8(q, layer, sealed, k, v, plan.address, plan.status, scale,
+                                        tail_row0, out, lse, need_lse)

@@ -45,6 +45,7 @@ class TilePlan:
         self.struct = N.Plan()
         N.check(lib.hsd_plan_init(C.c_void_p(base), nbytes, self.q_len, self.kv_len,
                                   C.byref(self.struct)), "hsd_plan_init")
+        self.address = C.addressof(self.struct)
         self.status = _dev_status(device)
         self.device = device
 

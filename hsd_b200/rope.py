@@ -111,7 +111,7 @@ class RotaryAxes:
                  device="cuda"):
         self.sections = [int(n) for n in sections]
         self.scaling = float(scaling)
-        axes = len(self.sections)
+        self.axes = axes = len(self.sections)
         if not 1 <= axes <= _MAX_AXES or min(self.sections) < 0 or sum(self.sections) != 64:
             raise ValueError(f"RotaryAxes: sections {self.sections} must be 1 to {_MAX_AXES} "
                              "counts that sum to 64 pairs")
@@ -137,29 +137,6 @@ class RotaryAxes:
                                   dtype=torch.int64, device=device)
         self.pair_axis = torch.tensor(axis, dtype=torch.int32, device=device)
 
-    @property
-    def axes(self):
-        return len(self.sections)
-
-
-def _positions(positions, axes, rows):
-    p = positions
-    if p.dim() == 3:  # [1, A, Q] or [A, 1, Q]
-        if p.shape[0] == 1:
-            p = p[0]
-        elif p.shape[1] == 1:
-            p = p[:, 0]
-    if p.dim() == 1 and axes == 1:
-        p = p[None]
-    if p.dim() != 2 or tuple(p.shape) != (axes, rows):
-        raise ValueError(f"rope_append_axes: positions {tuple(positions.shape)}, expected "
-                         f"[{axes}, {rows}]")
-    if p.dtype == torch.int32:
-        p = p.long()
-    if p.dtype != torch.int64 or not p.is_cuda:
-        raise TypeError("rope_append_axes: positions must be an int64 or int32 CUDA tensor")
-    return p
-
 
 def rope_append_axes(q, k, v, positions, rotary, k_cache, v_cache, dst_row0, out=None,
                      num_q_heads=None, num_kv_heads=None, status=None):
@@ -176,46 +153,6 @@ def rope_append_axes(q, k, v, positions, rotary, k_cache, v_cache, dst_row0, out
     Returns the rotated queries as a ``[1, Hq, Q, 128]`` view, or None when q
     is None.  Asynchronous on the device's current stream.
     """
-    kc, vc = _cache(k_cache, "k_cache"), _cache(v_cache, "v_cache")
-    hkv = num_kv_heads or kc.shape[0]
-    k2, v2 = _rows(k, "k", hkv * 128), _rows(v, "v", hkv * 128)
-    n = k2.shape[0]
-    if v2.shape[0] != n:
-        raise ValueError("rope_append_axes: k and v row counts differ")
-    if kc.stride() != vc.stride() or kc.shape != vc.shape or kc.shape[0] != hkv:
-        raise ValueError("rope_append_axes: k_cache and v_cache must have one layout")
-    if dst_row0 < 0 or dst_row0 + n > kc.shape[1]:
-        raise ValueError(f"rope_append_axes: rows {dst_row0}..{dst_row0 + n} past the cache")
-    pos = _positions(positions, rotary.axes, n)
-    hq, q2, o2 = 0, None, None
-    if q is not None:
-        hq = num_q_heads or q.shape[-1] // 128
-        q2 = _rows(q, "q", hq * 128)
-        o2 = q2 if out is None else _rows(out, "out", hq * 128)
-        if q2.shape[0] != n or o2.shape[0] != n:
-            raise ValueError("rope_append_axes: q, out and k row counts differ")
-        if out is not None and o2.data_ptr() != out.data_ptr():
-            raise ValueError("rope_append_axes: out must be rows of one stride")
-    elif out is not None:
-        raise ValueError("rope_append_axes: out without q")
-    dev = k2.device
-    tensors = (k2, v2, kc, vc, pos, rotary.turns, q2, o2)
-    if any(t is not None and t.device != dev for t in tensors):
-        raise ValueError("rope_append_axes: all tensors must be on one device")
-    if q2 is not None and out is None and q2.data_ptr() != q.data_ptr():
-        raise ValueError("rope_append_axes: q must be rows of one stride")
-    if kc.data_ptr() != k_cache.data_ptr() or vc.data_ptr() != v_cache.data_ptr():
-        raise ValueError("rope_append_axes: the caches must be views [..., Hkv, KV, 128]")
-    if n:
-        lib = N.load()
-        with torch.cuda.device(dev):
-            N.check(lib.hsd_rope_append_axes(
-                N.ptr(q2), 0 if q2 is None else q2.stride(0), N.ptr(o2),
-                0 if o2 is None else o2.stride(0), N.ptr(k2), k2.stride(0), N.ptr(v2),
-                v2.stride(0), N.ptr(pos), pos.stride(0), pos.stride(1), rotary.axes,
-                N.ptr(rotary.turns), N.ptr(rotary.pair_axis), rotary.scaling, n, hq, hkv, 128,
-                N.ptr(kc), kc.stride(0), N.ptr(vc), vc.stride(0), kc.stride(1), dst_row0,
-                N.ptr(status), N.stream_handle()), "hsd_rope_append_axes")
-    if q2 is None:
-        return None
-    return o2.unflatten(-1, (hq, 128)).unsqueeze(0).transpose(1, 2)
+    return N.ops().rope_append_axes(q, k, v, positions, rotary.turns, rotary.pair_axis,
+                                    rotary.axes, rotary.scaling, k_cache, v_cache, dst_row0, out,
+                                    num_q_heads, num_kv_heads, status)
