@@ -130,7 +130,8 @@ struct ManyLayout {
 ManyLayout many_layout(int32_t kv_len, int32_t hkv) {
   ManyLayout m;
   m.scales = hsd_host::kKv8FlagBytes + align256(hsd_host::attention_partials_bytes());
-  m.rows = m.scales + align256(size_t(hkv) * ((kv_len + 127) / 128) * 2 * sizeof(hsd::attn::ColumnScale));
+  m.rows = m.scales +
+           align256(size_t(hkv) * ((kv_len + 127) / 128) * 2 * sizeof(hsd::attn::ColumnScale));
   m.total = m.rows + size_t(2) * hkv * kv_len * hsd::kv8a::HD * 2;
   return m;
 }

@@ -5,28 +5,40 @@
 // one KV head are packed (packed row i = query row i / group, head i % group)
 // into tiles of 16, and the cache's columns are split over all SMs.  A warp
 // owns a running softmax of one tile and takes 64 sealed columns (or 32 bf16
-// ones) at a time: one TMA copy each of K and V, 8 KB each, into its own
-// two-stage ring; no warp waits for another before the join.
+// ones) at a time: one TMA copy each of K and V, 8 KB each, into its own three
+// buffers, each refilled as soon as its tile has been used; no warp waits for
+// another before the join.  At full rate a copy takes 3 to 4 us, so the SM needs
+// about 150 KB in flight: eight warps with three tiles each (with two tiles a
+// warp waited 870 of 6300 cycles for V).
 //
-// m16n8k16 bf16 MMAs (16 rows; tcgen05's smallest tile is 64 rows x 128
-// threads of softmax, mostly empty here).  The fragments come straight from
-// the bytes in shared memory: the order of dims inside an MMA's K = 16 is
-// free as long as Q agrees, and so is the order of columns as long as P and
-// the mask agree, so each lane's 16-byte load of K holds its operands of four
-// MMAs, and pairs of V rows are joined by byte permutes.  Columns 2t and
-// 2t + 1 of an S tile are columns t and t + 4 of its eight, and lane group g
-// holds V dims 16 perm(g)..+15, perm(n) = n / 2 + 4 (n % 2): with the 128-byte
-// swizzle every 16-byte load is then free of bank conflicts.
+// m16n8k16 MMAs (16 rows; tcgen05's smallest tile is 64 rows x 128 threads of
+// softmax, mostly empty here).  The fragments come straight from the bytes in
+// shared memory: the order of dims inside an MMA's K = 16 is free as long as Q
+// agrees, and so is the order of columns as long as P and the mask agree, so
+// each lane's 16-byte load of K holds its operands of four MMAs, and pairs of V
+// rows are joined by byte permutes.  Columns 2t and 2t + 1 of an S tile are
+// columns t and t + 4 of its eight, and lane group g holds V dims
+// 16 perm(g)..+15, perm(n) = n / 2 + 4 (n % 2): with the 128-byte swizzle
+// every 16-byte load is then free of bank conflicts.
 //
-// Scales: S is multiplied by the block's K scale inside the exponent; P by
-// the V scale before it is rounded to bf16 (bf16 keeps fp32's range, so no
-// scale underflows); the row sum takes the unrounded, unscaled P in fp32.
-// P's rounding (2^-9 relative, to nearest) is that of every bf16 attention.
+// Types.  Sealed columns run in fp16, where an int8 becomes a number with one
+// byte permute and one subtraction (1024 + 128 + n is the exponent byte above n's
+// byte, sign bit flipped) and P keeps 11 bits.  Ranges: each Q row is divided by
+// a power of two that brings its largest value to [1, 2) and enters the score
+// factor again; P is formed as 2^15 exp(s - max), so that weights down to
+// 2^-39 count; O is kept in units of the block's V scale and rescaled from
+// block to block.  bf16 columns run in bf16 throughout.  Scores, sums and O are
+// fp32; the row sum takes the unrounded P.
 //
-// Join: warps of a CTA through shared memory, CTAs through fp32 partial rows
-// in the workspace and a second small launch.  No counters and no flags: the
-// result does not depend on the order in which CTAs finish.
+// Join: warps of a CTA through shared memory; up to eight CTAs of a tile as a
+// cluster, each reading the others' rows from their shared memory; more through
+// fp32 partial rows in the workspace and a second small launch.  No counters
+// and no flags: the result does not depend on the order in which CTAs finish.
 #include "kv8_attn.cuh"
+
+#include <cuda_fp16.h>
+
+#include <atomic>
 
 namespace hsd {
 namespace kv8r {
@@ -34,26 +46,49 @@ namespace kv8r {
 using kv8a::HD;
 using kv8a::Params;
 
-constexpr int kWarps = 6;
+constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
-constexpr int kStages = 2;
-constexpr int kTile = 64 * HD;          // bytes: 64 int8 rows, or 32 bf16 rows
-constexpr int kStageBytes = 2 * kTile;  // K and V
+constexpr int kTile = 64 * HD;  // bytes: 64 int8 rows, or 32 bf16 rows
+constexpr int kBuf = 3;
+constexpr int kRing = kBuf * kTile;  // a warp's buffers: K, V, K, V, ... in turn
 constexpr int kRows = 16;
+constexpr int kMaxCluster = 8;
 constexpr int kRecord = kRows * HD + 2 * kRows;  // floats of a partial record
-constexpr size_t kSmem = size_t(kWarps) * kStages * kStageBytes + 1024;
+constexpr float kPShift = 15.0f;                 // P = 2^15 exp(s - max)
+
+struct __align__(1024) Smem {
+  uint8_t ring[kWarps][kRing];  // then each warp's O, rows HD + 4 floats apart
+  uint4 q16[8][32];             // Q fragments: fp16 of q / unit, and bf16
+  uint4 qbf[8][32];
+  float unit[kRows];  // power of two of the row
+  float2 ml[kWarps][kRows];
+  float2 cta_ml[kRows];  // the CTA's joined rows, for the other CTAs of the cluster
+  uint64_t full[kWarps][kBuf];
+  int abort;
+};
+constexpr size_t kSmem = sizeof(Smem) + 1024;
+static_assert(kSmem <= 232448, "shared memory budget exceeded");
+static_assert(kRows * (HD + 4) * 4 <= kRing, "a warp's O must fit its ring");
 
 struct Split {
-  float* partials;  // [tile][splits][kRecord], or null
+  float* partials;  // [tile][splits][kRecord], or null: one CTA or one cluster per tile
   int splits, n_tiles;
 };
 
 __device__ __forceinline__ int perm(int n) { return (n >> 1) | ((n & 1) << 2); }
 
-__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
-                                    uint32_t b1) {
+__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                         uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                        uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
       "{%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -68,116 +103,204 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   return v;
 }
 
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// Bytes `sel` (two nibble pairs) of a word of n + 128 -> two exact fp16.
+__device__ __forceinline__ uint32_t biased_to_f16(uint32_t w, uint32_t sel) {
+  uint32_t r;
+  const uint32_t p = __byte_perm(w, 0x64646464u, sel);
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(p), "r"(0x64806480u));  // 1152
+  return r;
+}
+// Four signed bytes -> two fp16 pairs.
+__device__ __forceinline__ void bytes_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  const uint32_t b = w ^ 0x80808080u;
+  lo = biased_to_f16(b, 0x4140);
+  hi = biased_to_f16(b, 0x4342);
+}
+
 // The warp's walk over its units: 64-column halves of the tile's block list,
-// a bf16 half in two steps of 32 columns.
-struct Cursor {
-  int u;        // half of the list, -1 before the first
-  int col;      // first column of the step
+// a bf16 half in two steps of 32 columns.  The list is read a unit ahead.
+struct Walk {
+  const uint32_t* list;
+  int n_units, stride, u;
+  uint32_t ahead;  // entry of unit u
+};
+struct Step {
+  int col;  // first column, -1: none
   bool tail, second, partial;
 };
 
-__device__ __forceinline__ bool next_step(const Params& p, const uint32_t* list, int n_units,
-                                          int stride, Cursor& c) {
-  if (c.tail && !c.second && c.col + 32 < p.kv_len) {
+__device__ __forceinline__ uint32_t list_entry(const Walk& w, int u) {
+  return u < w.n_units ? w.list[u >> 1] : 0u;
+}
+
+__device__ __forceinline__ Step next_step(const Params& p, Walk& w, const Step& last) {
+  Step c;
+  if (last.col >= 0 && last.tail && !last.second && last.col + 32 < p.kv_len) {
+    c = last;
     c.second = true;
     c.col += 32;
-    return true;
+    return c;
   }
+  c.second = false;
   while (true) {
-    c.u += stride;
-    if (c.u >= n_units) return false;
-    const uint32_t e = list[c.u >> 1];
-    const int hf = c.u & 1;
+    const uint32_t e = w.ahead;
+    const int u = w.u;
+    if (u >= w.n_units) {
+      c.col = -1;
+      c.tail = c.partial = false;
+      return c;
+    }
+    w.u += w.stride;
+    w.ahead = list_entry(w, w.u);
+    const int hf = u & 1;
     if (!((e >> (24 + 2 * hf)) & 1u)) continue;
     c.partial = ((e >> (25 + 2 * hf)) & 1u) != 0;
     c.col = int(e & 0xFFFFFFu) * 128 + 64 * hf;
     c.tail = c.col >= p.sealed;
-    c.second = false;
-    return true;
+    return c;
   }
 }
 
-// Running softmax of the warp's 16 rows; this lane: rows g and g + 8.
+// A step's scales and mask words (this lane's rows g and g + 8), loaded while
+// the step before is at its product.
+struct Aside {
+  float ks, vs;
+  uint64_t bits[2];
+};
+
+__device__ __forceinline__ void load_aside(const Params& p, const Step& c, int kvh, int qt,
+                                           const int (&mrow)[2], Aside& a) {
+  const int t64 = c.col >> 6;
+  a.ks = a.vs = 1.f;
+  if (!c.tail) {
+    a.ks = __ldg(p.k_scale + kvh * p.scale_stride + t64);
+    a.vs = __ldg(p.v_scale + kvh * p.scale_stride + t64);
+  }
+  a.bits[0] = a.bits[1] = ~0ull;
+  if (c.partial) {
+    const uint64_t* words = p.mask_words + (size_t(qt) * p.n_kv64 + t64) * 128;
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+      if (mrow[r] >= 0) a.bits[r] = words[mrow[r]];  // rows that do not exist mask nothing
+  }
+  if (c.second) {
+    a.bits[0] >>= 32;
+    a.bits[1] >>= 32;
+  }
+}
+
+// Running softmax of the warp's 16 rows; this lane: rows g and g + 8.  o is in
+// units of `unit` (0 before the first block), a V scale that blocks down to 2^-20
+// of it keep, their P carrying the quotient (fp16 P has room: weights down to
+// 2^-19 still count).  A block more than 2^60 below the largest scale so far does
+// not lower the unit further, so that O stays finite; its own part is then lost.
 struct State {
-  float m[2], l[2];
+  float m[2], l[2], unit, unit_max;
   float o[16][4];
 };
 
-// Scores of NT tiles of eight columns -> P (bf16 pairs) with the state
-// updated.  bits[r]: the row's mask, bit i = column i of the step.
-template <int NT>
+// Scores of NT tiles of eight columns -> P with the state's maximum, sum and
+// O brought up to date.
+template <int NT, bool kHalf>
 __device__ __forceinline__ void softmax_step(float (&c)[NT][4], const uint64_t (&bits)[2],
-                                             bool partial, float sc, float vs, int t, State& s,
-                                             uint32_t (&pk)[NT][2]) {
-  float mx[2] = {-INFINITY, -INFINITY};
+                                             bool masked, const float (&sc)[2], float vs, int t,
+                                             State& s, uint32_t (&pk)[NT][2]) {
+  s.unit_max = fmaxf(s.unit_max, vs);
+  const float low = fmaxf(vs, s.unit_max * 8.673617379884035e-19f);
+  const bool keep = vs <= s.unit && vs >= s.unit * 9.5367431640625e-07f;
+  const float v_unit = keep ? s.unit : low;
+  const float pv = __fdividef(vs, v_unit);
+  if (masked) {
 #pragma unroll
-  for (int j = 0; j < NT; ++j)
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      c[j][i] *= sc;
-      const int r = i >> 1;
-      if (partial && !((bits[r] >> (8 * j + t + 4 * (i & 1))) & 1ull)) c[j][i] = -INFINITY;
-      mx[r] = fmaxf(mx[r], c[j][i]);
-    }
+      for (int i = 0; i < 4; ++i)
+        if (!((uint32_t(bits[i >> 1] >> (8 * j)) >> (t + 4 * (i & 1))) & 1u)) c[j][i] = -INFINITY;
+  }
   float alpha[2], nm[2];
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
-    mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-    mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-    const float m_new = fmaxf(s.m[r], mx[r]);
-    nm[r] = m_new == -INFINITY ? 0.f : -m_new;
-    alpha[r] = ex2_approx(s.m[r] + nm[r]);  // 0 when the row had nothing yet
+    float mx = fmaxf(c[0][2 * r], c[0][2 * r + 1]);
+#pragma unroll
+    for (int j = 1; j < NT; ++j) mx = fmax3(mx, c[j][2 * r], c[j][2 * r + 1]);
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+    const float m_new = fmaxf(s.m[r], mx * sc[r]);
+    const float neg = m_new == -INFINITY ? 0.f : -m_new;
+    alpha[r] = ex2_approx(s.m[r] + neg);  // 0 when the row had nothing yet
+    nm[r] = neg + (kPShift + __log2f(pv));
     s.m[r] = m_new;
   }
-  float sum[2] = {0.f, 0.f};
+  // P with the quotient of the V scales; the row sum without it
+  const float unscale = __fdividef(v_unit, vs);
 #pragma unroll
-  for (int j = 0; j < NT; ++j)
+  for (int r = 0; r < 2; ++r) {
+    float sum0 = 0.f, sum1 = 0.f;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const float a = ex2_approx(c[j][2 * r] + nm[r]);
-      const float b = ex2_approx(c[j][2 * r + 1] + nm[r]);
-      sum[r] += a + b;
-      pk[j][r] = pack_bf16x2(a * vs, b * vs);
+    for (int j = 0; j < NT; ++j) {
+      const float a = ex2_approx(fmaf(c[j][2 * r], sc[r], nm[r]));
+      const float b = ex2_approx(fmaf(c[j][2 * r + 1], sc[r], nm[r]));
+      sum0 += a;
+      sum1 += b;
+      pk[j][r] = kHalf ? pack_f16x2(a, b) : pack_bf16x2(a, b);
     }
-  s.l[0] = s.l[0] * alpha[0] + sum[0];
-  s.l[1] = s.l[1] * alpha[1] + sum[1];
-  if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+    s.l[r] = s.l[r] * alpha[r] + (sum0 + sum1) * unscale;
+  }
+  const float f = __fdividef(s.unit, v_unit);
+  s.unit = v_unit;
+  const float f0 = alpha[0] * f, f1 = alpha[1] * f;
+  if (__any_sync(0xffffffffu, f0 != 1.f || f1 != 1.f)) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      s.o[i][0] *= alpha[0];
-      s.o[i][1] *= alpha[0];
-      s.o[i][2] *= alpha[1];
-      s.o[i][3] *= alpha[1];
+      s.o[i][0] *= f0;
+      s.o[i][1] *= f0;
+      s.o[i][2] *= f1;
+      s.o[i][3] *= f1;
     }
   }
 }
 
-__device__ __forceinline__ void sealed_step(uint32_t kb, uint32_t vb, const uint32_t (&qf)[8][4],
-                                            const uint64_t (&bits)[2], bool partial, float sc,
-                                            float vs, int g, int t, State& s) {
-  float c[8][4];
-  const int pg = perm(g);
+__device__ __forceinline__ void sealed_scores(uint32_t kb, const uint4 (*q16)[32], int g, int t,
+                                              float (&c)[8][4]) {
+  const int pg = perm(g), lane = lane_id();
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
+  for (int j = 0; j < 8; ++j)
 #pragma unroll
     for (int i = 0; i < 4; ++i) c[j][i] = 0.f;
-    const uint32_t row = kb + uint32_t(8 * j + pg) * 128u;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint4 w = lds128(row + (uint32_t((4 * h + t) ^ pg) << 4));
-      uint32_t b0, b1;
-      kv8a::bytes_to_bf16(w.x, b0, b1);
-      mma(c[j], qf[4 * h], b0, b1);
-      kv8a::bytes_to_bf16(w.y, b0, b1);
-      mma(c[j], qf[4 * h + 1], b0, b1);
-      kv8a::bytes_to_bf16(w.z, b0, b1);
-      mma(c[j], qf[4 * h + 2], b0, b1);
-      kv8a::bytes_to_bf16(w.w, b0, b1);
-      mma(c[j], qf[4 * h + 3], b0, b1);
+  for (int h = 0; h < 2; ++h) {
+    uint32_t w[8][4];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint4 v = lds128(kb + uint32_t(8 * j + pg) * 128u + (uint32_t((4 * h + t) ^ pg) << 4));
+      w[j][0] = v.x;
+      w[j][1] = v.y;
+      w[j][2] = v.z;
+      w[j][3] = v.w;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint4 qv = q16[4 * h + k][lane];
+      const uint32_t a[4] = {qv.x, qv.y, qv.z, qv.w};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        uint32_t b0, b1;
+        bytes_to_f16(w[j][k], b0, b1);
+        mma_f16(c[j], a, b0, b1);
+      }
     }
   }
-  uint32_t pk[8][2];
-  softmax_step<8>(c, bits, partial, sc, vs, t, s, pk);
+}
+
+__device__ __forceinline__ void sealed_values(uint32_t vb, const uint32_t (&pk)[8][2], int g, int t,
+                                              State& s) {
+  const int pg = perm(g);
 #pragma unroll
   for (int kk = 0; kk < 4; ++kk) {
     const uint32_t a[4] = {pk[2 * kk][0], pk[2 * kk][1], pk[2 * kk + 1][0], pk[2 * kk + 1][1]};
@@ -186,51 +309,54 @@ __device__ __forceinline__ void sealed_step(uint32_t kb, uint32_t vb, const uint
     for (int i = 0; i < 4; ++i) {
       const int r = 16 * kk + 4 * i + t;
       const uint4 v = lds128(vb + uint32_t(r) * 128u + (uint32_t(pg ^ (r & 7)) << 4));
-      w[i][0] = v.x;
-      w[i][1] = v.y;
-      w[i][2] = v.z;
-      w[i][3] = v.w;
+      w[i][0] = v.x ^ 0x80808080u;
+      w[i][1] = v.y ^ 0x80808080u;
+      w[i][2] = v.z ^ 0x80808080u;
+      w[i][3] = v.w ^ 0x80808080u;
     }
 #pragma unroll
     for (int d = 0; d < 4; ++d) {
-      uint32_t x0, x1, x2, x3, y0, y1, y2, y3;
-      kv8a::bytes_to_bf16(__byte_perm(w[0][d], w[1][d], 0x5140), x0, x1);
-      kv8a::bytes_to_bf16(__byte_perm(w[0][d], w[1][d], 0x7362), x2, x3);
-      kv8a::bytes_to_bf16(__byte_perm(w[2][d], w[3][d], 0x5140), y0, y1);
-      kv8a::bytes_to_bf16(__byte_perm(w[2][d], w[3][d], 0x7362), y2, y3);
-      mma(s.o[4 * d], a, x0, y0);
-      mma(s.o[4 * d + 1], a, x1, y1);
-      mma(s.o[4 * d + 2], a, x2, y2);
-      mma(s.o[4 * d + 3], a, x3, y3);
+      const uint32_t x = __byte_perm(w[0][d], w[1][d], 0x5140);
+      const uint32_t y = __byte_perm(w[0][d], w[1][d], 0x7362);
+      const uint32_t u = __byte_perm(w[2][d], w[3][d], 0x5140);
+      const uint32_t v = __byte_perm(w[2][d], w[3][d], 0x7362);
+      mma_f16(s.o[4 * d], a, biased_to_f16(x, 0x4140), biased_to_f16(u, 0x4140));
+      mma_f16(s.o[4 * d + 1], a, biased_to_f16(x, 0x4342), biased_to_f16(u, 0x4342));
+      mma_f16(s.o[4 * d + 2], a, biased_to_f16(y, 0x4140), biased_to_f16(v, 0x4140));
+      mma_f16(s.o[4 * d + 3], a, biased_to_f16(y, 0x4342), biased_to_f16(v, 0x4342));
     }
   }
 }
 
 // 32 bf16 columns: two 64-dim sub-tiles of 32 rows x 128 bytes per operand.
-// V rows that no row of the tile sees (seen) read as zero, so what stands in
-// masked columns never reaches the sums.
-__device__ __forceinline__ void tail_step(uint32_t kb, uint32_t vb, const uint32_t (&qf)[8][4],
-                                          const uint64_t (&bits)[2], bool partial, uint32_t seen,
-                                          float sc, int g, int t, State& s) {
-  float c[4][4];
-  const int pg = perm(g);
+__device__ __forceinline__ void tail_scores(uint32_t kb, const uint4 (*qbf)[32], int g, int t,
+                                            float (&c)[4][4]) {
+  const int pg = perm(g), lane = lane_id();
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
+  for (int j = 0; j < 4; ++j)
 #pragma unroll
     for (int i = 0; i < 4; ++i) c[j][i] = 0.f;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t row = kb + uint32_t(h * (kTile / 2) + (8 * j + pg) * 128);
+  for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int cc = 0; cc < 2; ++cc) {
-        const uint4 w = lds128(row + (uint32_t((2 * t + cc) ^ pg) << 4));
-        mma(c[j], qf[4 * h + 2 * cc], w.x, w.y);
-        mma(c[j], qf[4 * h + 2 * cc + 1], w.z, w.w);
+    for (int cc = 0; cc < 2; ++cc) {
+      const uint4 q0 = qbf[4 * h + 2 * cc][lane], q1 = qbf[4 * h + 2 * cc + 1][lane];
+      const uint32_t a0[4] = {q0.x, q0.y, q0.z, q0.w}, a1[4] = {q1.x, q1.y, q1.z, q1.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint4 w = lds128(kb + uint32_t(h * (kTile / 2) + (8 * j + pg) * 128) +
+                               (uint32_t((2 * t + cc) ^ pg) << 4));
+        mma_bf16(c[j], a0, w.x, w.y);
+        mma_bf16(c[j], a1, w.z, w.w);
       }
     }
-  }
-  uint32_t pk[4][2];
-  softmax_step<4>(c, bits, partial, sc, 1.f, t, s, pk);
+}
+
+// V rows that no row of the tile sees (seen) read as zero, so what stands in
+// masked columns never reaches the sums.
+__device__ __forceinline__ void tail_values(uint32_t vb, const uint32_t (&pk)[4][2], uint32_t seen,
+                                            int g, int t, State& s) {
+  const int pg = perm(g);
   const uint32_t vsub = vb + uint32_t((pg >> 2) * (kTile / 2));
 #pragma unroll
   for (int kk = 0; kk < 2; ++kk) {
@@ -251,10 +377,10 @@ __device__ __forceinline__ void tail_step(uint32_t kb, uint32_t vb, const uint32
       }
 #pragma unroll
       for (int d = 0; d < 4; ++d) {
-        mma(s.o[8 * cc + 2 * d], a, __byte_perm(w[0][d], w[1][d], 0x5410),
-            __byte_perm(w[2][d], w[3][d], 0x5410));
-        mma(s.o[8 * cc + 2 * d + 1], a, __byte_perm(w[0][d], w[1][d], 0x7632),
-            __byte_perm(w[2][d], w[3][d], 0x7632));
+        mma_bf16(s.o[8 * cc + 2 * d], a, __byte_perm(w[0][d], w[1][d], 0x5410),
+                 __byte_perm(w[2][d], w[3][d], 0x5410));
+        mma_bf16(s.o[8 * cc + 2 * d + 1], a, __byte_perm(w[0][d], w[1][d], 0x7632),
+                 __byte_perm(w[2][d], w[3][d], 0x7632));
       }
     }
   }
@@ -268,7 +394,68 @@ __device__ __forceinline__ void store_row(const Params& p, int kvh, int row, int
       make_uint2(pack_bf16x2(v.x * inv, v.y * inv), pack_bf16x2(v.z * inv, v.w * inv));
   if (d4 == 0 && p.lse)
     p.lse[size_t(h) * p.q_len + q] =
-        l > 0.f ? (m + __log2f(l)) * 0.69314718055994530942f : -INFINITY;
+        l > 0.f ? (m - kPShift + __log2f(l)) * 0.69314718055994530942f : -INFINITY;
+}
+
+// Q rows of the tile in MMA fragment order: MMA 4 h + w covers dims
+// 64 h + 16 t + 4 w..+3 of lane group t; words: row g dims 0-1, row g + 8 dims
+// 0-1, row g dims 2-3, row g + 8 dims 2-3.
+__device__ __forceinline__ void stage_q(const Params& p, Smem& sm, int kvh, int row0, int n_rows) {
+  const int tid = threadIdx.x;
+  if (tid >= kRows * 16) return;
+  const int r = tid >> 4, c = tid & 15;  // 8 dims
+  uint4 v = make_uint4(0u, 0u, 0u, 0u);
+  if (r < n_rows) {
+    const int i = row0 + r, q = i / p.group;
+    v = *reinterpret_cast<const uint4*>(p.q + int64_t(q) * p.q_row_stride +
+                                        int64_t(kvh * p.group + i - q * p.group) *
+                                            p.q_head_stride + 8 * c);
+  }
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) top = __vmaxu2(top, w[i] & 0x7FFF7FFFu);
+  top = max(top & 0xFFFFu, top >> 16);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  // the power of two at or below the row's largest |q|, as a float's exponent
+  const uint32_t e = min(max((top & 0x7F80u) << 16, 27u << 23), 227u << 23);
+  const float inv = __uint_as_float((254u << 23) - e);
+  if (c == 0) sm.unit[r] = __uint_as_float(e);
+  const int h = c >> 3, t = (c & 7) >> 1, k0 = 4 * h + 2 * (c & 1);
+  const int lane = (r & 7) * 4 + t, hi = r >> 3;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {  // dims 8 c + 2 i, + 1: MMA k0 + i / 2, pair i % 2
+    const float a = __uint_as_float(w[i] << 16) * inv;
+    const float b = __uint_as_float(w[i] & 0xFFFF0000u) * inv;
+    reinterpret_cast<uint32_t*>(&sm.q16[k0 + (i >> 1)][lane])[2 * (i & 1) + hi] = pack_f16x2(a, b);
+    reinterpret_cast<uint32_t*>(&sm.qbf[k0 + (i >> 1)][lane])[2 * (i & 1) + hi] = w[i];
+  }
+}
+
+__device__ __forceinline__ uint32_t cluster_addr(const void* p, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float4 ld_cluster_v4(uint32_t a) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(a)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 ld_cluster_v2(uint32_t a) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
+               : "=f"(v.x), "=f"(v.y)
+               : "r"(a)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
 
 // CTA (split, KV head, tile of 16 packed rows)
@@ -277,136 +464,134 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const __grid_constant__ CUtensorMap tm_kt, const __grid_constant__ CUtensorMap tm_vt,
                 const Params p, const Split sp) {
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
-                                             ~uintptr_t(1023));
-  __shared__ uint64_t full[kWarps][kStages];
-  __shared__ float2 ml[kWarps][kRows];
-  __shared__ int abort_flag;
+  Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                      ~uintptr_t(1023));
   const int warp = warp_id(), lane = lane_id();
   const int g = lane >> 2, t = lane & 3;
-  if (threadIdx.x == 0) {
-    for (int w = 0; w < kWarps; ++w)
-      for (int i = 0; i < kStages; ++i) mbar_init(&full[w][i], 1);
-    abort_flag = 0;
-    fence_barrier_init();
-  }
-  __syncthreads();
+  if (threadIdx.x == 0) sm.abort = 0;
+  if (lane < kBuf) mbar_init(&sm.full[warp][lane], 1);
+  fence_barrier_init();
+  __syncwarp();
   pdl_wait_then_release();  // launched with launch_pdl: nothing global is read before
-  volatile int* abort = &abort_flag;
+  volatile int* abort = &sm.abort;
   const int kvh = blockIdx.y;
   const int row0 = int(blockIdx.z) * kRows;  // first packed row
   const int n_rows = min(kRows, p.q_len * p.group - row0);
   const int qt = (row0 / p.group) >> 7;  // a tile's rows lie in one query tile: 128 group % 16 == 0
-  const uint32_t* list = p.blk_list + size_t(qt) * p.n_kv128;
-  const int n_units = 2 * p.blk_count[qt];
-  const int stride = sp.splits * kWarps;
-  uint8_t* ring = smem + warp * (kStages * kStageBytes);
-
-  Cursor ic;  // issued up to here
-  ic.u = int(blockIdx.x) * kWarps + warp - stride;
-  ic.tail = ic.second = ic.partial = false;
-  ic.col = 0;
-  Cursor cc = ic;  // consumed up to here
-  int issued = 0, consumed = 0;
-  auto issue = [&]() {
-    if (!next_step(p, list, n_units, stride, ic)) return;
+  Walk walk;
+  walk.list = p.blk_list + size_t(qt) * p.n_kv128;
+  walk.n_units = 2 * p.blk_count[qt];
+  walk.stride = sp.splits * kWarps;
+  walk.u = int(blockIdx.x) * kWarps + warp;
+  walk.ahead = list_entry(walk, walk.u);
+  uint8_t* ring = sm.ring[warp];
+  // operand tile i (K of step n: 2 n, V: 2 n + 1) into buffer i % kBuf
+  int issued = 0;
+  int fill = 0;  // issued % kBuf
+  auto issue = [&](const Step& c, bool is_v) {
     if (lane == 0) {
-      uint64_t* bar = &full[warp][issued % kStages];
-      uint8_t* kd = ring + (issued % kStages) * kStageBytes;
-      uint8_t* vd = kd + kTile;
-      mbar_arrive_expect_tx(bar, kStageBytes);
-      if (ic.tail) {
-        const int r = ic.col - p.tail_row0;
-        for (int h = 0; h < 2; ++h) {
-          tma_load_3d(kd + h * (kTile / 2), &tm_kt, bar, 64 * h, r, kvh);
-          tma_load_3d(vd + h * (kTile / 2), &tm_vt, bar, 64 * h, r, kvh);
-        }
+      uint64_t* bar = &sm.full[warp][fill];
+      uint8_t* dst = ring + fill * kTile;
+      mbar_arrive_expect_tx(bar, kTile);
+      if (c.tail) {
+        for (int h = 0; h < 2; ++h)
+          tma_load_3d(dst + h * (kTile / 2), is_v ? &tm_vt : &tm_kt, bar, 64 * h,
+                      c.col - p.tail_row0, kvh);
       } else {
-        tma_load_3d(kd, &tm_k8, bar, 0, ic.col, kvh);
-        tma_load_3d(vd, &tm_v8, bar, 0, ic.col, kvh);
+        tma_load_3d(dst, is_v ? &tm_v8 : &tm_k8, bar, 0, c.col, kvh);
       }
     }
     ++issued;
+    fill = fill + 1 == kBuf ? 0 : fill + 1;
   };
-  for (int i = 0; i < kStages; ++i) issue();
-
-  // Q fragments: MMA (h, w) covers dims 64 h + 16 t + 4 w..+3 of lane group t
-  uint32_t qf[8][4];
+  Step none;
+  none.col = -1;
+  none.tail = none.second = none.partial = false;
+  Step cur = next_step(p, walk, none);
+  Step nxt = none;
+  if (cur.col >= 0) {
+    issue(cur, false);
+    issue(cur, true);
+    nxt = next_step(p, walk, cur);
+    if (nxt.col >= 0) issue(nxt, false);
+  }
   int mrow[2];  // the lane's rows in the query tile, -1: no such row
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const int i = row0 + g + 8 * r;
-    const bool have = g + 8 * r < n_rows;
-    const int q = i / p.group;
-    mrow[r] = have ? (q & 127) : -1;
-    const __nv_bfloat16* src = p.q + int64_t(q) * p.q_row_stride +
-                               int64_t(kvh * p.group + i - q * p.group) * p.q_head_stride;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint4 a = make_uint4(0u, 0u, 0u, 0u), b = a;
-      if (have) {
-        a = *reinterpret_cast<const uint4*>(src + 64 * h + 16 * t);
-        b = *reinterpret_cast<const uint4*>(src + 64 * h + 16 * t + 8);
-      }
-      qf[4 * h][r] = a.x;
-      qf[4 * h][r + 2] = a.y;
-      qf[4 * h + 1][r] = a.z;
-      qf[4 * h + 1][r + 2] = a.w;
-      qf[4 * h + 2][r] = b.x;
-      qf[4 * h + 2][r + 2] = b.y;
-      qf[4 * h + 3][r] = b.z;
-      qf[4 * h + 3][r + 2] = b.w;
-    }
-  }
+  for (int r = 0; r < 2; ++r)
+    mrow[r] = g + 8 * r < n_rows ? ((row0 + g + 8 * r) / p.group) & 127 : -1;
+  Aside a;  // of the current step
+  if (cur.col >= 0) load_aside(p, cur, kvh, qt, mrow, a);
+  stage_q(p, sm, kvh, row0, n_rows);
+  __syncthreads();  // Q fragments and the abort word
 
   State s;
   s.m[0] = s.m[1] = -INFINITY;
   s.l[0] = s.l[1] = 0.f;
+  s.unit = s.unit_max = 0.f;
 #pragma unroll
   for (int i = 0; i < 16; ++i)
 #pragma unroll
     for (int k = 0; k < 4; ++k) s.o[i][k] = 0.f;
 
+  int used = 0;  // tiles used
+  int at = 0;    // used % kBuf
+  uint32_t parity = 0;
   bool ok = true;
-  while (ok && next_step(p, list, n_units, stride, cc)) {
-    const int tile64 = cc.col >> 6;
-    float sc = p.scale_log2, vs = 1.f;
-    if (!cc.tail) {
-      sc *= p.k_scale[kvh * p.scale_stride + tile64];
-      vs = p.v_scale[kvh * p.scale_stride + tile64];
+  auto wait_tile = [&](int32_t where) {
+    ok = __all_sync(0xffffffffu, mbar_wait(&sm.full[warp][at], parity, abort, p.status, where));
+    return ok;
+  };
+  auto done_tile = [&]() {  // every lane has read the tile
+    __syncwarp();
+    ++used;
+    if (++at == kBuf) {
+      at = 0;
+      parity ^= 1u;
     }
-    uint64_t bits[2] = {~0ull, ~0ull};
-    uint32_t seen = 0xffffffffu;
-    if (cc.partial) {
-      const uint64_t* words = p.mask_words + (size_t(qt) * p.n_kv64 + tile64) * 128;
-      bits[0] = mrow[0] >= 0 ? words[mrow[0]] : 0ull;
-      bits[1] = mrow[1] >= 0 ? words[mrow[1]] : 0ull;
+  };
+  while (cur.col >= 0) {
+    Step after = none;  // the step after next
+    if (nxt.col >= 0) after = next_step(p, walk, nxt);
+    const bool masked = __any_sync(0xffffffffu, (a.bits[0] & a.bits[1]) != ~0ull);
+    const bool any = !masked || __any_sync(0xffffffffu, (a.bits[0] | a.bits[1]) != 0ull);
+    if (!wait_tile(0x800)) break;
+    // one step of 64 sealed or 32 bf16 columns
+    if (cur.tail) {
+      float c[4][4];
+      tail_scores(smem_u32(ring + at * kTile), sm.qbf, g, t, c);
+      done_tile();
+      if (nxt.col >= 0) issue(nxt, true);
+      uint32_t pk[4][2];
+      const float sc[2] = {p.scale_log2, p.scale_log2};
+      if (any) softmax_step<4, false>(c, a.bits, masked, sc, 1.f, t, s, pk);
+      // columns that some existing row sees
+      const uint32_t seen = __reduce_or_sync(
+          0xffffffffu, (mrow[0] >= 0 ? uint32_t(a.bits[0]) : 0u) |
+                           (mrow[1] >= 0 ? uint32_t(a.bits[1]) : 0u));
+      if (nxt.col >= 0) load_aside(p, nxt, kvh, qt, mrow, a);
+      if (!wait_tile(0x801)) break;
+      if (any) tail_values(smem_u32(ring + at * kTile), pk, seen, g, t, s);
+    } else {
+      float c[8][4];
+      sealed_scores(smem_u32(ring + at * kTile), sm.q16, g, t, c);
+      done_tile();
+      if (nxt.col >= 0) issue(nxt, true);
+      uint32_t pk[8][2];
+      const float f = p.scale_log2 * a.ks;
+      const float sc[2] = {f * sm.unit[g], f * sm.unit[g + 8]};
+      if (any) softmax_step<8, true>(c, a.bits, masked, sc, a.vs, t, s, pk);
+      if (nxt.col >= 0) load_aside(p, nxt, kvh, qt, mrow, a);
+      if (!wait_tile(0x802)) break;
+      if (any) sealed_values(smem_u32(ring + at * kTile), pk, g, t, s);
     }
-    if (cc.tail) {
-      if (cc.second) {
-        bits[0] >>= 32;
-        bits[1] >>= 32;
-      }
-      seen = __reduce_or_sync(0xffffffffu, uint32_t(bits[0]) | uint32_t(bits[1]));
-    }
-    const int st = consumed % kStages;
-    ok = __all_sync(0xffffffffu, mbar_wait(&full[warp][st], uint32_t(consumed / kStages) & 1u,
-                                           abort, p.status, 0x800));
-    if (!ok) break;
-    const uint32_t kb = smem_u32(ring + st * kStageBytes);
-    if (!cc.partial || __any_sync(0xffffffffu, (bits[0] | bits[1]) != 0ull)) {
-      if (cc.tail)
-        tail_step(kb, kb + kTile, qf, bits, cc.partial, seen, sc, g, t, s);
-      else
-        sealed_step(kb, kb + kTile, qf, bits, cc.partial, sc, vs, g, t, s);
-    }
-    ++consumed;
-    __syncwarp();  // every lane has read the stage before it is refilled
-    issue();
+    done_tile();
+    if (after.col >= 0) issue(after, false);
+    cur = nxt;
+    nxt = after;
   }
   if (!ok)  // copies in flight must land before the CTA's memory goes
-    for (int k = consumed; k < issued; ++k)
-      mbar_wait(&full[warp][k % kStages], uint32_t(k / kStages) & 1u, abort, p.status, 0x801,
+    for (; used < issued; ++used)
+      mbar_wait(&sm.full[warp][used % kBuf], uint32_t(used / kBuf) & 1u, abort, p.status, 0x803,
                 false);
 
   // ---- join the CTA's warps
@@ -414,34 +599,34 @@ __global__ void __launch_bounds__(kThreads, 1)
   for (int r = 0; r < 2; ++r) {
     s.l[r] += __shfl_xor_sync(0xffffffffu, s.l[r], 1);
     s.l[r] += __shfl_xor_sync(0xffffffffu, s.l[r], 2);
-    if (t == 0) ml[warp][g + 8 * r] = make_float2(s.m[r], s.l[r]);
+    if (t == 0) sm.ml[warp][g + 8 * r] = make_float2(s.m[r], s.l[r]);
     float* dst = reinterpret_cast<float*>(ring) + (g + 8 * r) * (HD + 4);
 #pragma unroll
     for (int e = 0; e < 2; ++e)
 #pragma unroll
       for (int i = 0; i < 16; i += 4)
         *reinterpret_cast<float4*>(dst + 64 * e + 16 * t + i) =
-            make_float4(s.o[i][2 * r + e], s.o[i + 1][2 * r + e], s.o[i + 2][2 * r + e],
-                        s.o[i + 3][2 * r + e]);
+            make_float4(s.o[i][2 * r + e] * s.unit, s.o[i + 1][2 * r + e] * s.unit,
+                        s.o[i + 2][2 * r + e] * s.unit, s.o[i + 3][2 * r + e] * s.unit);
   }
   __syncthreads();
   const size_t tile = size_t(kvh) * gridDim.z + blockIdx.z;
   float* rec = sp.partials ? sp.partials + (tile * sp.splits + blockIdx.x) * kRecord : nullptr;
+  const bool cluster = sp.splits > 1 && !rec;
   for (int idx = threadIdx.x; idx < n_rows * 32; idx += kThreads) {
     const int r = idx >> 5, d4 = idx & 31;
     float m = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, ml[w][r].x);
+    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, sm.ml[w][r].x);
     const float nm = m == -INFINITY ? 0.f : -m;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     float l = 0.f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float2 x = ml[w][r];
+      const float2 x = sm.ml[w][r];
       const float f = ex2_approx(x.x + nm);
       const float4 v = *reinterpret_cast<const float4*>(
-          reinterpret_cast<const float*>(smem + w * (kStages * kStageBytes)) + r * (HD + 4) +
-          4 * d4);
+          reinterpret_cast<const float*>(sm.ring[w]) + r * (HD + 4) + 4 * d4);
       l += x.y * f;
       acc.x += v.x * f;
       acc.y += v.y * f;
@@ -451,34 +636,104 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (rec) {
       *reinterpret_cast<float4*>(rec + r * HD + 4 * d4) = acc;
       if (d4 == 0) reinterpret_cast<float2*>(rec + kRows * HD)[r] = make_float2(m, l);
+    } else if (cluster) {
+      // each element is read and written by this thread alone
+      *reinterpret_cast<float4*>(reinterpret_cast<float*>(sm.ring[0]) + r * (HD + 4) + 4 * d4) =
+          acc;
+      if (d4 == 0) sm.cta_ml[r] = make_float2(m, l);
     } else {
       store_row(p, kvh, row0 + r, d4, acc, m, l);
     }
   }
+  if (!cluster) return;
+  // ---- join the cluster's CTAs: rows dealt out, each read from every CTA
+  cluster_sync();
+  for (int r = int(blockIdx.x) + sp.splits * warp; r < n_rows; r += sp.splits * kWarps) {
+    float m = -INFINITY;
+    for (int k = 0; k < sp.splits; ++k)
+      m = fmaxf(m, ld_cluster_v2(cluster_addr(&sm.cta_ml[r], uint32_t(k))).x);
+    const float nm = m == -INFINITY ? 0.f : -m;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.f;
+#pragma unroll 4
+    for (int k = 0; k < sp.splits; ++k) {
+      const float2 x = ld_cluster_v2(cluster_addr(&sm.cta_ml[r], uint32_t(k)));
+      const float4 v = ld_cluster_v4(cluster_addr(
+          reinterpret_cast<const float*>(sm.ring[0]) + r * (HD + 4) + 4 * lane, uint32_t(k)));
+      const float f = ex2_approx(x.x + nm);
+      l += x.y * f;
+      acc.x += v.x * f;
+      acc.y += v.y * f;
+      acc.z += v.z * f;
+      acc.w += v.w * f;
+    }
+    store_row(p, kvh, row0 + r, lane, acc, m, l);
+  }
+  cluster_sync();  // no CTA leaves while another reads its rows
 }
 
-// Join the splits: warp (packed row, KV head), lane = 4 dims.
-__global__ void __launch_bounds__(128) join_kernel(const Params p, const Split sp) {
+// Join the splits: CTA (packed row, KV head), its warps the splits in turn, lane
+// = 4 dims.
+constexpr int kJoinWarps = 8;
+__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const Params p, const Split sp) {
   pdl_wait_then_release();  // launched with launch_pdl
-  const int row = int(blockIdx.x) * 4 + warp_id();
-  const int kvh = blockIdx.y, d4 = lane_id();
-  if (row >= p.q_len * p.group) return;
+  __shared__ float4 acc_s[kJoinWarps][32];
+  __shared__ float2 ml_s[kJoinWarps];
+  const int row = blockIdx.x, kvh = blockIdx.y, warp = warp_id(), d4 = lane_id();
   const int r = row % kRows;
-  const float* rec0 =
-      sp.partials + (size_t(kvh) * sp.n_tiles + row / kRows) * sp.splits * kRecord;
-  float m = -INFINITY;
-  for (int i = d4; i < sp.splits; i += 32)
-    m = fmaxf(m, __ldcg(rec0 + size_t(i) * kRecord + kRows * HD + 2 * r));
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const float nm = m == -INFINITY ? 0.f : -m;
+  const float* rec0 = sp.partials + (size_t(kvh) * sp.n_tiles + row / kRows) * sp.splits * kRecord;
+  float m = -INFINITY, l = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float l = 0.f;
-#pragma unroll 8
-  for (int i = 0; i < sp.splits; ++i) {
-    const float* rec = rec0 + size_t(i) * kRecord;
-    const float2 x = __ldcg(reinterpret_cast<const float2*>(rec + kRows * HD) + r);
-    const float4 v = __ldcg(reinterpret_cast<const float4*>(rec + r * HD) + d4);
+  constexpr int kAt = 8;  // records in flight
+  for (int i0 = warp; i0 < sp.splits; i0 += kJoinWarps * kAt) {
+    float2 x[kAt];
+    float4 v[kAt];
+#pragma unroll
+    for (int k = 0; k < kAt; ++k) {
+      const int i = i0 + k * kJoinWarps;
+      x[k] = make_float2(-INFINITY, 0.f);
+      v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i < sp.splits) {
+        const float* rec = rec0 + size_t(i) * kRecord;
+        x[k] = __ldcg(reinterpret_cast<const float2*>(rec + kRows * HD) + r);
+        v[k] = __ldcg(reinterpret_cast<const float4*>(rec + r * HD) + d4);
+      }
+    }
+    float m_new = m;
+#pragma unroll
+    for (int k = 0; k < kAt; ++k) m_new = fmaxf(m_new, x[k].x);
+    const float nm = m_new == -INFINITY ? 0.f : -m_new;
+    const float a = ex2_approx(m + nm);
+    l *= a;
+    acc.x *= a;
+    acc.y *= a;
+    acc.z *= a;
+    acc.w *= a;
+#pragma unroll
+    for (int k = 0; k < kAt; ++k) {
+      const float f = ex2_approx(x[k].x + nm);
+      l += x[k].y * f;
+      acc.x += v[k].x * f;
+      acc.y += v[k].y * f;
+      acc.z += v[k].z * f;
+      acc.w += v[k].w * f;
+    }
+    m = m_new;
+  }
+  acc_s[warp][d4] = acc;
+  if (d4 == 0) ml_s[warp] = make_float2(m, l);
+  __syncthreads();
+  if (warp > 0) return;
+  float top = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, ml_s[w].x);
+  const float nm = top == -INFINITY ? 0.f : -top;
+  l = 0.f;
+  acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) {
+    const float2 x = ml_s[w];
+    const float4 v = acc_s[w][d4];
     const float f = ex2_approx(x.x + nm);
     l += x.y * f;
     acc.x += v.x * f;
@@ -486,7 +741,7 @@ __global__ void __launch_bounds__(128) join_kernel(const Params p, const Split s
     acc.z += v.z * f;
     acc.w += v.w * f;
   }
-  store_row(p, kvh, row, d4, acc, m, l);
+  store_row(p, kvh, row, d4, acc, top, l);
 }
 
 }  // namespace kv8r
@@ -497,10 +752,14 @@ namespace hsd_host {
 using namespace hsd;
 
 namespace {
+constexpr int kMaxDevices = 64;
+std::atomic<bool> g_attr_set[kMaxDevices];
+
 int n_tiles(int q_len, int group) {
   return int((int64_t(q_len) * group + kv8r::kRows - 1) / kv8r::kRows);
 }
-// CTAs per tile: one wave of one CTA per SM, each warp with a unit at least.
+// CTAs per tile: one wave of one CTA per SM, each warp with a unit at least;
+// up to kMaxCluster of them are a cluster.
 int n_splits(int q_len, int kv_len, int hq, int hkv) {
   const int64_t tiles = int64_t(n_tiles(q_len, hq / hkv)) * hkv;
   const int units = (kv_len + 63) / 64;
@@ -512,7 +771,7 @@ int n_splits(int q_len, int kv_len, int hq, int hkv) {
 
 size_t kv8_rows_workspace_bytes(int q_len, int kv_len, int hq, int hkv) {
   const int s = n_splits(q_len, kv_len, hq, hkv);
-  if (s == 1) return kKv8FlagBytes;
+  if (s <= kv8r::kMaxCluster) return kKv8FlagBytes;
   return kKv8FlagBytes + size_t(n_tiles(q_len, hq / hkv)) * hkv * s * kv8r::kRecord * sizeof(float);
 }
 
@@ -578,26 +837,38 @@ int kv8_rows_launch(const Kv8AttnArgs& a) {
   kv8r::Split sp;
   sp.n_tiles = n_tiles(p.q_len, p.group);
   sp.splits = n_splits(p.q_len, p.kv_len, p.hq, p.hkv);
-  sp.partials = sp.splits > 1 ? reinterpret_cast<float*>(static_cast<char*>(a.workspace) + kKv8FlagBytes)
-                               : nullptr;
+  const bool cluster = sp.splits > 1 && sp.splits <= kv8r::kMaxCluster;
+  sp.partials = sp.splits > kv8r::kMaxCluster
+                    ? reinterpret_cast<float*>(static_cast<char*>(a.workspace) + kKv8FlagBytes)
+                    : nullptr;
   if (sp.n_tiles > 65535 || p.hkv > 65535) {
     set_error("hsd_verify_attention_kv8: %d rows x %d heads exceed the launch's range", p.q_len,
               p.hq);
     return HSD_ERR_TOO_LARGE;
   }
-  rc = cuda_check(cudaFuncSetAttribute(kv8r::rows_kernel,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       int(kv8r::kSmem)),
-                  "cudaFuncSetAttribute(rows_kernel)");
+  int dev = 0;
+  rc = cuda_check(cudaGetDevice(&dev), "cudaGetDevice");
   if (rc) return rc;
+  if (dev < 0 || dev >= kMaxDevices) {
+    set_error("hsd_verify_attention_kv8: device ordinal %d >= %d", dev, kMaxDevices);
+    return HSD_ERR_UNSUPPORTED;
+  }
+  if (!g_attr_set[dev].load(std::memory_order_acquire)) {
+    rc = cuda_check(cudaFuncSetAttribute(kv8r::rows_kernel,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         int(kv8r::kSmem)),
+                    "cudaFuncSetAttribute(rows_kernel)");
+    if (rc) return rc;
+    g_attr_set[dev].store(true, std::memory_order_release);
+  }
   rc = launch_pdl(kv8r::rows_kernel,
                   dim3(unsigned(sp.splits), unsigned(p.hkv), unsigned(sp.n_tiles)),
-                  dim3(kv8r::kThreads), kv8r::kSmem, a.stream, "rows_kernel launch", 0, k8, v8, kt,
-                  vt, p, sp);
-  if (rc || sp.splits == 1) return rc;
+                  dim3(kv8r::kThreads), kv8r::kSmem, a.stream, "rows_kernel launch",
+                  cluster ? unsigned(sp.splits) : 0u, k8, v8, kt, vt, p, sp);
+  if (rc || !sp.partials) return rc;
   return launch_pdl(kv8r::join_kernel,
-                    dim3(unsigned((p.q_len * p.group + 3) / 4), unsigned(p.hkv)), dim3(128), 0,
-                    a.stream, "join_kernel launch", 0, p, sp);
+                    dim3(unsigned(p.q_len * p.group), unsigned(p.hkv)),
+                    dim3(kv8r::kJoinWarps * 32), 0, a.stream, "join_kernel launch", 0, p, sp);
 }
 
 }  // namespace hsd_host
