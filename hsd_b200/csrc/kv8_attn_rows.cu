@@ -11,15 +11,18 @@
 // about 150 KB in flight: eight warps with three tiles each (with two tiles a
 // warp waited 870 of 6300 cycles for V).
 //
-// m16n8k16 MMAs (16 rows; tcgen05's smallest tile is 64 rows x 128 threads of
-// softmax, mostly empty here).  The fragments come straight from the bytes in
-// shared memory: the order of dims inside an MMA's K = 16 is free as long as Q
-// agrees, and so is the order of columns as long as P and the mask agree, so
-// each lane's 16-byte load of K holds its operands of four MMAs, and pairs of V
-// rows are joined by byte permutes.  Columns 2t and 2t + 1 of an S tile are
-// columns t and t + 4 of its eight, and lane group g holds V dims
-// 16 perm(g)..+15, perm(n) = n / 2 + 4 (n % 2): with the 128-byte swizzle
-// every 16-byte load is then free of bank conflicts.
+// m16n8k16 MMAs (tcgen05's smallest tile is 64 rows with a thread of softmax
+// each, mostly empty here), transposed: S^T = K Q^T and O^T = V^T P^T, so that
+// the cache fills the 16-row side and 8 or 16 query rows (kNB = 1 or 2 blocks of
+// 8) the other: with 8 rows, half the MMAs and accumulators of the upright form.
+// The fragments come straight from the bytes in shared memory: the order of dims
+// inside an MMA's K = 16 is free as long as Q agrees, and so is the order of
+// columns as long as P and the mask agree, so each lane's 16-byte load of K holds
+// its operands of four MMAs, and pairs of V rows are joined by byte permutes; P^T
+// needs one 8 x 8 transpose (movmatrix) per 8 columns.  Column n of eight is
+// column perm(n) = n / 2 + 4 (n % 2), and lane group g holds V dims
+// 16 perm(g)..+15: with the 128-byte swizzle every 16-byte load is then free of
+// bank conflicts.
 //
 // Types.  Sealed columns run in fp16, where an int8 becomes a number with one
 // byte permute and one subtraction (1024 + 128 + n is the exponent byte above n's
@@ -49,58 +52,52 @@ using kv8a::Params;
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
 constexpr int kTile = 64 * HD;  // bytes: 64 int8 rows, or 32 bf16 rows
-constexpr int kBuf = 3;
+constexpr int kBuf = 3;  // the issue order keeps exactly three tiles ahead
+static_assert(kBuf == 3, "a step's K and V and the next step's K are issued before any is used");
 constexpr int kRing = kBuf * kTile;  // a warp's buffers: K, V, K, V, ... in turn
-constexpr int kRows = 16;
+constexpr int kMaxRows = 16;
 constexpr int kMaxCluster = 8;
-constexpr int kRecord = kRows * HD + 2 * kRows;  // floats of a partial record
+constexpr int kRecord = kMaxRows * HD + 2 * kMaxRows;  // floats of a partial record
 constexpr float kPShift = 15.0f;                 // P = 2^15 exp(s - max)
 
 struct __align__(1024) Smem {
   uint8_t ring[kWarps][kRing];  // then each warp's O, rows HD + 4 floats apart
-  uint4 q16[8][32];             // Q fragments: fp16 of q / unit, and bf16
-  uint4 qbf[8][32];
-  float unit[kRows];  // power of two of the row
-  float2 ml[kWarps][kRows];
-  float2 cta_ml[kRows];  // the CTA's joined rows, for the other CTAs of the cluster
+  uint2 q16[8][2][32];          // Q fragments [MMA][block of 8 rows]: fp16 of q / unit, bf16
+  uint2 qbf[8][2][32];
+  float unit[kMaxRows];  // power of two of the row
+  float2 ml[kWarps][kMaxRows];
+  float2 cta_ml[kMaxRows];  // the CTA's joined rows, for the other CTAs of the cluster
   uint64_t full[kWarps][kBuf];
   int abort;
 };
 constexpr size_t kSmem = sizeof(Smem) + 1024;
 static_assert(kSmem <= 232448, "shared memory budget exceeded");
-static_assert(kRows * (HD + 4) * 4 <= kRing, "a warp's O must fit its ring");
+static_assert(kMaxRows * (HD + 4) * 4 <= kRing, "a warp's O must fit its ring");
 
 struct Split {
   float* partials;  // [tile][splits][kRecord], or null: one CTA or one cluster per tile
-  int splits, n_tiles;
+  int splits, n_tiles, rows;  // rows: packed rows of a tile
 };
 
 __device__ __forceinline__ int perm(int n) { return (n >> 1) | ((n & 1) << 2); }
 
 __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
                                          uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
       "{%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
                                         uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
       "{%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ uint4 lds128(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "r"(addr)
-               : "memory");
-  return v;
+__device__ __forceinline__ uint4 lds128(const uint8_t* p) {
+  return *reinterpret_cast<const uint4*>(p);
 }
 
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
@@ -167,118 +164,139 @@ __device__ __forceinline__ Step next_step(const Params& p, Walk& w, const Step& 
   }
 }
 
-// A step's scales and mask words (this lane's rows g and g + 8), loaded while
-// the step before is at its product.
+__device__ __forceinline__ uint32_t transpose8(uint32_t a) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+
+// A step's scales and mask words (this lane's rows 2 t and 2 t + 1 of each block
+// of 8), loaded while the step before is at its product.
+template <int kNB>
 struct Aside {
   float ks, vs;
-  uint64_t bits[2];
+  uint64_t bits[2 * kNB];
 };
 
+template <int kNB>
 __device__ __forceinline__ void load_aside(const Params& p, const Step& c, int kvh, int qt,
-                                           const int (&mrow)[2], Aside& a) {
+                                           const int (&mrow)[2 * kNB], Aside<kNB>& a) {
   const int t64 = c.col >> 6;
   a.ks = a.vs = 1.f;
   if (!c.tail) {
     a.ks = __ldg(p.k_scale + kvh * p.scale_stride + t64);
     a.vs = __ldg(p.v_scale + kvh * p.scale_stride + t64);
   }
-  a.bits[0] = a.bits[1] = ~0ull;
-  if (c.partial) {
-    const uint64_t* words = p.mask_words + (size_t(qt) * p.n_kv64 + t64) * 128;
+  const uint64_t* words = p.mask_words + (size_t(qt) * p.n_kv64 + t64) * 128;
 #pragma unroll
-    for (int r = 0; r < 2; ++r)
-      if (mrow[r] >= 0) a.bits[r] = words[mrow[r]];  // rows that do not exist mask nothing
-  }
-  if (c.second) {
-    a.bits[0] >>= 32;
-    a.bits[1] >>= 32;
+  for (int r = 0; r < 2 * kNB; ++r) {
+    a.bits[r] = ~0ull;  // rows that do not exist mask nothing
+    if (c.partial && mrow[r] >= 0) a.bits[r] = words[mrow[r]];
+    if (c.second) a.bits[r] >>= 32;
   }
 }
 
-// Running softmax of the warp's 16 rows; this lane: rows g and g + 8.  o is in
-// units of `unit` (0 before the first block), a V scale that blocks down to 2^-20
-// of it keep, their P carrying the quotient (fp16 P has room: weights down to
-// 2^-19 still count).  A block more than 2^60 below the largest scale so far does
-// not lower the unit further, so that O stays finite; its own part is then lost.
+// Running softmax of the warp's 8 kNB rows; this lane: rows 2 t and 2 t + 1 of
+// each block.  o is in units of `unit` (0 before the first block), a V scale that
+// blocks down to 2^-20 of it keep, their P carrying the quotient (fp16 P has room:
+// weights down to 2^-19 still count).  A block more than 2^60 below the largest
+// scale so far does not lower the unit further, so that O stays finite; its own
+// part is then lost.
+template <int kNB>
 struct State {
-  float m[2], l[2], unit, unit_max;
-  float o[16][4];
+  float m[2 * kNB], l[2 * kNB], unit, unit_max;
+  float o[kNB][8][4];  // dims 16 perm(g) + 2 i, + 1 of rows 2 t, 2 t + 1
 };
 
-// Scores of NT tiles of eight columns -> P with the state's maximum, sum and
-// O brought up to date.
-template <int NT, bool kHalf>
-__device__ __forceinline__ void softmax_step(float (&c)[NT][4], const uint64_t (&bits)[2],
-                                             bool masked, const float (&sc)[2], float vs, int t,
-                                             State& s, uint32_t (&pk)[NT][2]) {
+// Scores of NT tiles of 16 columns (c: column perm(g), rows 2 t and 2 t + 1, then
+// column 8 + perm(g)) -> P^T fragments, with the state's maximum, sum and O
+// brought up to date.
+template <int kNB, int NT, bool kHalf>
+__device__ __forceinline__ void softmax_step(float (&c)[kNB][NT][4],
+                                             const uint64_t (&bits)[2 * kNB], bool masked,
+                                             const float (&sc)[2 * kNB], float vs, int pg,
+                                             State<kNB>& s, uint32_t (&pk)[kNB][NT][2]) {
   s.unit_max = fmaxf(s.unit_max, vs);
   const float low = fmaxf(vs, s.unit_max * 8.673617379884035e-19f);
   const bool keep = vs <= s.unit && vs >= s.unit * 9.5367431640625e-07f;
   const float v_unit = keep ? s.unit : low;
-  const float pv = __fdividef(vs, v_unit);
   if (masked) {
+#pragma unroll
+    for (int b = 0; b < kNB; ++b)
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (!((uint32_t(bits[2 * b + (i & 1)] >> (16 * j)) >> (pg + 8 * (i >> 1))) & 1u))
+            c[b][j][i] = -INFINITY;
+  }
+  const float shift = kPShift + __log2f(__fdividef(vs, v_unit));
+  // P with the quotient of the V scales; the row sum without it
+  const float unscale = __fdividef(v_unit, vs);
+  const float f = __fdividef(s.unit, v_unit);
+  s.unit = v_unit;
+  float of[2 * kNB];  // factors on O
+  bool any = false;
+#pragma unroll
+  for (int b = 0; b < kNB; ++b) {
+    float nm[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = 2 * b + e;
+      float mx = fmaxf(c[b][0][e], c[b][0][2 + e]);
+#pragma unroll
+      for (int j = 1; j < NT; ++j) mx = fmax3(mx, c[b][j][e], c[b][j][2 + e]);
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      const float m_new = fmaxf(s.m[r], mx * sc[r]);
+      const float neg = m_new == -INFINITY ? 0.f : -m_new;
+      const float alpha = ex2_approx(s.m[r] + neg);  // 0 when the row had nothing yet
+      nm[e] = neg + shift;
+      s.m[r] = m_new;
+      of[r] = alpha * f;
+      any |= of[r] != 1.f;
+      s.l[r] *= alpha;
+    }
+    float sum[2] = {0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (!((uint32_t(bits[i >> 1] >> (8 * j)) >> (t + 4 * (i & 1))) & 1u)) c[j][i] = -INFINITY;
+      for (int k = 0; k < 2; ++k) {
+        const float x = ex2_approx(fmaf(c[b][j][2 * k], sc[2 * b], nm[0]));
+        const float y = ex2_approx(fmaf(c[b][j][2 * k + 1], sc[2 * b + 1], nm[1]));
+        sum[0] += x;
+        sum[1] += y;
+        pk[b][j][k] = transpose8(kHalf ? pack_f16x2(x, y) : pack_bf16x2(x, y));
+      }
+    s.l[2 * b] += sum[0] * unscale;
+    s.l[2 * b + 1] += sum[1] * unscale;
   }
-  float alpha[2], nm[2];
+  if (__any_sync(0xffffffffu, any)) {
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    float mx = fmaxf(c[0][2 * r], c[0][2 * r + 1]);
+    for (int b = 0; b < kNB; ++b)
 #pragma unroll
-    for (int j = 1; j < NT; ++j) mx = fmax3(mx, c[j][2 * r], c[j][2 * r + 1]);
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-    const float m_new = fmaxf(s.m[r], mx * sc[r]);
-    const float neg = m_new == -INFINITY ? 0.f : -m_new;
-    alpha[r] = ex2_approx(s.m[r] + neg);  // 0 when the row had nothing yet
-    nm[r] = neg + (kPShift + __log2f(pv));
-    s.m[r] = m_new;
-  }
-  // P with the quotient of the V scales; the row sum without it
-  const float unscale = __fdividef(v_unit, vs);
+      for (int i = 0; i < 8; ++i)
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    float sum0 = 0.f, sum1 = 0.f;
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const float a = ex2_approx(fmaf(c[j][2 * r], sc[r], nm[r]));
-      const float b = ex2_approx(fmaf(c[j][2 * r + 1], sc[r], nm[r]));
-      sum0 += a;
-      sum1 += b;
-      pk[j][r] = kHalf ? pack_f16x2(a, b) : pack_bf16x2(a, b);
-    }
-    s.l[r] = s.l[r] * alpha[r] + (sum0 + sum1) * unscale;
-  }
-  const float f = __fdividef(s.unit, v_unit);
-  s.unit = v_unit;
-  const float f0 = alpha[0] * f, f1 = alpha[1] * f;
-  if (__any_sync(0xffffffffu, f0 != 1.f || f1 != 1.f)) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      s.o[i][0] *= f0;
-      s.o[i][1] *= f0;
-      s.o[i][2] *= f1;
-      s.o[i][3] *= f1;
-    }
+        for (int k = 0; k < 4; ++k) s.o[b][i][k] *= of[2 * b + (k & 1)];
   }
 }
 
-__device__ __forceinline__ void sealed_scores(uint32_t kb, const uint4 (*q16)[32], int g, int t,
-                                              float (&c)[8][4]) {
+template <int kNB>
+__device__ __forceinline__ void sealed_scores(const uint8_t* kb, const uint2 (*q16)[2][32], int g,
+                                              int t, float (&c)[kNB][4][4]) {
   const int pg = perm(g), lane = lane_id();
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
+  for (int b = 0; b < kNB; ++b)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) c[j][i] = 0.f;
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c[b][j][i] = 0.f;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    uint32_t w[8][4];
+    uint32_t w[8][4];  // column perm(g) of eight times eight
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const uint4 v = lds128(kb + uint32_t(8 * j + pg) * 128u + (uint32_t((4 * h + t) ^ pg) << 4));
+      const uint4 v = lds128(kb + (8 * j + pg) * 128 + (((4 * h + t) ^ pg) << 4));
       w[j][0] = v.x;
       w[j][1] = v.y;
       w[j][2] = v.z;
@@ -286,29 +304,32 @@ __device__ __forceinline__ void sealed_scores(uint32_t kb, const uint4 (*q16)[32
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const uint4 qv = q16[4 * h + k][lane];
-      const uint32_t a[4] = {qv.x, qv.y, qv.z, qv.w};
+      uint2 q[kNB];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        uint32_t b0, b1;
-        bytes_to_f16(w[j][k], b0, b1);
-        mma_f16(c[j], a, b0, b1);
+      for (int b = 0; b < kNB; ++b) q[b] = q16[4 * h + k][b][lane];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t a[4];
+        bytes_to_f16(w[2 * j][k], a[0], a[2]);
+        bytes_to_f16(w[2 * j + 1][k], a[1], a[3]);
+#pragma unroll
+        for (int b = 0; b < kNB; ++b) mma_f16(c[b][j], a, q[b].x, q[b].y);
       }
     }
   }
 }
 
-__device__ __forceinline__ void sealed_values(uint32_t vb, const uint32_t (&pk)[8][2], int g, int t,
-                                              State& s) {
+template <int kNB>
+__device__ __forceinline__ void sealed_values(const uint8_t* vb, const uint32_t (&pk)[kNB][4][2],
+                                              int g, int t, State<kNB>& s) {
   const int pg = perm(g);
 #pragma unroll
   for (int kk = 0; kk < 4; ++kk) {
-    const uint32_t a[4] = {pk[2 * kk][0], pk[2 * kk][1], pk[2 * kk + 1][0], pk[2 * kk + 1][1]};
     uint32_t w[4][4];  // rows t, t + 4, t + 8, t + 12 of the 16: dims 16 pg..+15
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int r = 16 * kk + 4 * i + t;
-      const uint4 v = lds128(vb + uint32_t(r) * 128u + (uint32_t(pg ^ (r & 7)) << 4));
+      const uint4 v = lds128(vb + r * 128 + ((pg ^ (r & 7)) << 4));
       w[i][0] = v.x ^ 0x80808080u;
       w[i][1] = v.y ^ 0x80808080u;
       w[i][2] = v.z ^ 0x80808080u;
@@ -316,59 +337,64 @@ __device__ __forceinline__ void sealed_values(uint32_t vb, const uint32_t (&pk)[
     }
 #pragma unroll
     for (int d = 0; d < 4; ++d) {
-      const uint32_t x = __byte_perm(w[0][d], w[1][d], 0x5140);
-      const uint32_t y = __byte_perm(w[0][d], w[1][d], 0x7362);
-      const uint32_t u = __byte_perm(w[2][d], w[3][d], 0x5140);
-      const uint32_t v = __byte_perm(w[2][d], w[3][d], 0x7362);
-      mma_f16(s.o[4 * d], a, biased_to_f16(x, 0x4140), biased_to_f16(u, 0x4140));
-      mma_f16(s.o[4 * d + 1], a, biased_to_f16(x, 0x4342), biased_to_f16(u, 0x4342));
-      mma_f16(s.o[4 * d + 2], a, biased_to_f16(y, 0x4140), biased_to_f16(v, 0x4140));
-      mma_f16(s.o[4 * d + 3], a, biased_to_f16(y, 0x4342), biased_to_f16(v, 0x4342));
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {  // dims 4 d + 2 e, + 1
+        const uint32_t lo = __byte_perm(w[0][d], w[1][d], e ? 0x7362 : 0x5140);
+        const uint32_t hi = __byte_perm(w[2][d], w[3][d], e ? 0x7362 : 0x5140);
+        const uint32_t a[4] = {biased_to_f16(lo, 0x4140), biased_to_f16(lo, 0x4342),
+                               biased_to_f16(hi, 0x4140), biased_to_f16(hi, 0x4342)};
+#pragma unroll
+        for (int b = 0; b < kNB; ++b) mma_f16(s.o[b][2 * d + e], a, pk[b][kk][0], pk[b][kk][1]);
+      }
     }
   }
 }
 
 // 32 bf16 columns: two 64-dim sub-tiles of 32 rows x 128 bytes per operand.
-__device__ __forceinline__ void tail_scores(uint32_t kb, const uint4 (*qbf)[32], int g, int t,
-                                            float (&c)[4][4]) {
+template <int kNB>
+__device__ __forceinline__ void tail_scores(const uint8_t* kb, const uint2 (*qbf)[2][32], int g,
+                                            int t, float (&c)[kNB][2][4]) {
   const int pg = perm(g), lane = lane_id();
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
+  for (int b = 0; b < kNB; ++b)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) c[j][i] = 0.f;
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c[b][j][i] = 0.f;
 #pragma unroll
   for (int h = 0; h < 2; ++h)
 #pragma unroll
-    for (int cc = 0; cc < 2; ++cc) {
-      const uint4 q0 = qbf[4 * h + 2 * cc][lane], q1 = qbf[4 * h + 2 * cc + 1][lane];
-      const uint32_t a0[4] = {q0.x, q0.y, q0.z, q0.w}, a1[4] = {q1.x, q1.y, q1.z, q1.w};
+    for (int cc = 0; cc < 2; ++cc)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint4 w = lds128(kb + uint32_t(h * (kTile / 2) + (8 * j + pg) * 128) +
-                               (uint32_t((2 * t + cc) ^ pg) << 4));
-        mma_bf16(c[j], a0, w.x, w.y);
-        mma_bf16(c[j], a1, w.z, w.w);
+      for (int j = 0; j < 2; ++j) {
+        const uint8_t* row = kb + h * (kTile / 2) + (16 * j + pg) * 128 + (((2 * t + cc) ^ pg) << 4);
+        const uint4 x = lds128(row), y = lds128(row + 8 * 128);
+        const uint32_t a0[4] = {x.x, y.x, x.y, y.y}, a1[4] = {x.z, y.z, x.w, y.w};
+#pragma unroll
+        for (int b = 0; b < kNB; ++b) {
+          const uint2 q0 = qbf[4 * h + 2 * cc][b][lane], q1 = qbf[4 * h + 2 * cc + 1][b][lane];
+          mma_bf16(c[b][j], a0, q0.x, q0.y);
+          mma_bf16(c[b][j], a1, q1.x, q1.y);
+        }
       }
-    }
 }
 
 // V rows that no row of the tile sees (seen) read as zero, so what stands in
 // masked columns never reaches the sums.
-__device__ __forceinline__ void tail_values(uint32_t vb, const uint32_t (&pk)[4][2], uint32_t seen,
-                                            int g, int t, State& s) {
+template <int kNB>
+__device__ __forceinline__ void tail_values(const uint8_t* vb, const uint32_t (&pk)[kNB][2][2],
+                                            uint32_t seen, int g, int t, State<kNB>& s) {
   const int pg = perm(g);
-  const uint32_t vsub = vb + uint32_t((pg >> 2) * (kTile / 2));
+  const uint8_t* vsub = vb + (pg >> 2) * (kTile / 2);
 #pragma unroll
-  for (int kk = 0; kk < 2; ++kk) {
-    const uint32_t a[4] = {pk[2 * kk][0], pk[2 * kk][1], pk[2 * kk + 1][0], pk[2 * kk + 1][1]};
+  for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
     for (int cc = 0; cc < 2; ++cc) {
       uint32_t w[4][4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int r = 16 * kk + 4 * i + t;
-        uint4 v = lds128(vsub + uint32_t(r) * 128u +
-                         (uint32_t((2 * (pg & 3) + cc) ^ (r & 7)) << 4));
+        uint4 v = lds128(vsub + r * 128 + (((2 * (pg & 3) + cc) ^ (r & 7)) << 4));
         if (!((seen >> r) & 1u)) v = make_uint4(0u, 0u, 0u, 0u);
         w[i][0] = v.x;
         w[i][1] = v.y;
@@ -376,14 +402,15 @@ __device__ __forceinline__ void tail_values(uint32_t vb, const uint32_t (&pk)[4]
         w[i][3] = v.w;
       }
 #pragma unroll
-      for (int d = 0; d < 4; ++d) {
-        mma_bf16(s.o[8 * cc + 2 * d], a, __byte_perm(w[0][d], w[1][d], 0x5410),
-                 __byte_perm(w[2][d], w[3][d], 0x5410));
-        mma_bf16(s.o[8 * cc + 2 * d + 1], a, __byte_perm(w[0][d], w[1][d], 0x7632),
-                 __byte_perm(w[2][d], w[3][d], 0x7632));
+      for (int d = 0; d < 4; ++d) {  // dims 8 cc + 2 d, + 1
+        const uint32_t a[4] = {__byte_perm(w[0][d], w[1][d], 0x5410),
+                               __byte_perm(w[0][d], w[1][d], 0x7632),
+                               __byte_perm(w[2][d], w[3][d], 0x5410),
+                               __byte_perm(w[2][d], w[3][d], 0x7632)};
+#pragma unroll
+        for (int b = 0; b < kNB; ++b) mma_bf16(s.o[b][4 * cc + d], a, pk[b][kk][0], pk[b][kk][1]);
       }
     }
-  }
 }
 
 __device__ __forceinline__ void store_row(const Params& p, int kvh, int row, int d4, float4 v,
@@ -398,11 +425,11 @@ __device__ __forceinline__ void store_row(const Params& p, int kvh, int row, int
 }
 
 // Q rows of the tile in MMA fragment order: MMA 4 h + w covers dims
-// 64 h + 16 t + 4 w..+3 of lane group t; words: row g dims 0-1, row g + 8 dims
-// 0-1, row g dims 2-3, row g + 8 dims 2-3.
+// 64 h + 16 t + 4 w..+3 of lane group t; lane 4 g + t has row g of the block.
+template <int kNB>
 __device__ __forceinline__ void stage_q(const Params& p, Smem& sm, int kvh, int row0, int n_rows) {
   const int tid = threadIdx.x;
-  if (tid >= kRows * 16) return;
+  if (tid >= 8 * kNB * 16) return;
   const int r = tid >> 4, c = tid & 15;  // 8 dims
   uint4 v = make_uint4(0u, 0u, 0u, 0u);
   if (r < n_rows) {
@@ -423,13 +450,16 @@ __device__ __forceinline__ void stage_q(const Params& p, Smem& sm, int kvh, int 
   const float inv = __uint_as_float((254u << 23) - e);
   if (c == 0) sm.unit[r] = __uint_as_float(e);
   const int h = c >> 3, t = (c & 7) >> 1, k0 = 4 * h + 2 * (c & 1);
-  const int lane = (r & 7) * 4 + t, hi = r >> 3;
+  const int lane = (r & 7) * 4 + t, block = r >> 3;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {  // dims 8 c + 2 i, + 1: MMA k0 + i / 2, pair i % 2
-    const float a = __uint_as_float(w[i] << 16) * inv;
-    const float b = __uint_as_float(w[i] & 0xFFFF0000u) * inv;
-    reinterpret_cast<uint32_t*>(&sm.q16[k0 + (i >> 1)][lane])[2 * (i & 1) + hi] = pack_f16x2(a, b);
-    reinterpret_cast<uint32_t*>(&sm.qbf[k0 + (i >> 1)][lane])[2 * (i & 1) + hi] = w[i];
+  for (int i = 0; i < 2; ++i) {  // dims 8 c + 4 i..+3: MMA k0 + i
+    uint32_t f[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      f[k] = pack_f16x2(__uint_as_float(w[2 * i + k] << 16) * inv,
+                        __uint_as_float(w[2 * i + k] & 0xFFFF0000u) * inv);
+    sm.q16[k0 + i][block][lane] = make_uint2(f[0], f[1]);
+    sm.qbf[k0 + i][block][lane] = make_uint2(w[2 * i], w[2 * i + 1]);
   }
 }
 
@@ -458,16 +488,17 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
 
-// CTA (split, KV head, tile of 16 packed rows)
+// CTA (split, KV head, tile of 8 kNB packed rows)
+template <int kNB>
 __global__ void __launch_bounds__(kThreads, 1)
     rows_kernel(const __grid_constant__ CUtensorMap tm_k8, const __grid_constant__ CUtensorMap tm_v8,
                 const __grid_constant__ CUtensorMap tm_kt, const __grid_constant__ CUtensorMap tm_vt,
                 const Params p, const Split sp) {
-  extern __shared__ uint8_t smem_raw[];
-  Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
-                                      ~uintptr_t(1023));
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  // (offset from the array, so that the compiler knows these are shared loads)
+  Smem& sm = *reinterpret_cast<Smem*>(smem_raw + ((0u - smem_u32(smem_raw)) & 1023u));
   const int warp = warp_id(), lane = lane_id();
-  const int g = lane >> 2, t = lane & 3;
+  const int g = lane >> 2, t = lane & 3, pg = perm(g);
   if (threadIdx.x == 0) sm.abort = 0;
   if (lane < kBuf) mbar_init(&sm.full[warp][lane], 1);
   fence_barrier_init();
@@ -475,9 +506,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_wait_then_release();  // launched with launch_pdl: nothing global is read before
   volatile int* abort = &sm.abort;
   const int kvh = blockIdx.y;
+  constexpr int kRows = 8 * kNB;
   const int row0 = int(blockIdx.z) * kRows;  // first packed row
   const int n_rows = min(kRows, p.q_len * p.group - row0);
-  const int qt = (row0 / p.group) >> 7;  // a tile's rows lie in one query tile: 128 group % 16 == 0
+  // a tile's rows lie in one query tile: 128 group is a multiple of 16
+  const int qt = (row0 / p.group) >> 7;
   Walk walk;
   walk.list = p.blk_list + size_t(qt) * p.n_kv128;
   walk.n_units = 2 * p.blk_count[qt];
@@ -515,23 +548,32 @@ __global__ void __launch_bounds__(kThreads, 1)
     nxt = next_step(p, walk, cur);
     if (nxt.col >= 0) issue(nxt, false);
   }
-  int mrow[2];  // the lane's rows in the query tile, -1: no such row
+  int mrow[2 * kNB];  // the lane's rows in the query tile, -1: no such row
 #pragma unroll
-  for (int r = 0; r < 2; ++r)
-    mrow[r] = g + 8 * r < n_rows ? ((row0 + g + 8 * r) / p.group) & 127 : -1;
-  Aside a;  // of the current step
-  if (cur.col >= 0) load_aside(p, cur, kvh, qt, mrow, a);
-  stage_q(p, sm, kvh, row0, n_rows);
+  for (int r = 0; r < 2 * kNB; ++r) {
+    const int i = 8 * (r >> 1) + 2 * t + (r & 1);
+    mrow[r] = i < n_rows ? ((row0 + i) / p.group) & 127 : -1;
+  }
+  Aside<kNB> a;  // of the current step
+  if (cur.col >= 0) load_aside<kNB>(p, cur, kvh, qt, mrow, a);
+  stage_q<kNB>(p, sm, kvh, row0, n_rows);
   __syncthreads();  // Q fragments and the abort word
 
-  State s;
-  s.m[0] = s.m[1] = -INFINITY;
-  s.l[0] = s.l[1] = 0.f;
+  State<kNB> s;
   s.unit = s.unit_max = 0.f;
+  float q_unit[2 * kNB];  // the rows' score factors
 #pragma unroll
-  for (int i = 0; i < 16; ++i)
+  for (int r = 0; r < 2 * kNB; ++r) {
+    s.m[r] = -INFINITY;
+    s.l[r] = 0.f;
+    q_unit[r] = p.scale_log2 * sm.unit[8 * (r >> 1) + 2 * t + (r & 1)];
+  }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) s.o[i][k] = 0.f;
+  for (int b = 0; b < kNB; ++b)
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s.o[b][i][k] = 0.f;
 
   int used = 0;  // tiles used
   int at = 0;    // used % kBuf
@@ -552,37 +594,45 @@ __global__ void __launch_bounds__(kThreads, 1)
   while (cur.col >= 0) {
     Step after = none;  // the step after next
     if (nxt.col >= 0) after = next_step(p, walk, nxt);
-    const bool masked = __any_sync(0xffffffffu, (a.bits[0] & a.bits[1]) != ~0ull);
-    const bool any = !masked || __any_sync(0xffffffffu, (a.bits[0] | a.bits[1]) != 0ull);
+    uint64_t all = ~0ull, some = 0ull;
+#pragma unroll
+    for (int r = 0; r < 2 * kNB; ++r) {
+      all &= a.bits[r];
+      if (mrow[r] >= 0) some |= a.bits[r];
+    }
+    if (cur.tail) all |= 0xffffffff00000000ull;
+    const bool masked = __any_sync(0xffffffffu, all != ~0ull);
+    const bool any = !masked || __any_sync(0xffffffffu, some != 0ull);
     if (!wait_tile(0x800)) break;
     // one step of 64 sealed or 32 bf16 columns
     if (cur.tail) {
-      float c[4][4];
-      tail_scores(smem_u32(ring + at * kTile), sm.qbf, g, t, c);
+      float c[kNB][2][4];
+      tail_scores<kNB>(ring + at * kTile, sm.qbf, g, t, c);
       done_tile();
       if (nxt.col >= 0) issue(nxt, true);
-      uint32_t pk[4][2];
-      const float sc[2] = {p.scale_log2, p.scale_log2};
-      if (any) softmax_step<4, false>(c, a.bits, masked, sc, 1.f, t, s, pk);
-      // columns that some existing row sees
-      const uint32_t seen = __reduce_or_sync(
-          0xffffffffu, (mrow[0] >= 0 ? uint32_t(a.bits[0]) : 0u) |
-                           (mrow[1] >= 0 ? uint32_t(a.bits[1]) : 0u));
-      if (nxt.col >= 0) load_aside(p, nxt, kvh, qt, mrow, a);
+      uint32_t pk[kNB][2][2];
+      float sc[2 * kNB];
+#pragma unroll
+      for (int r = 0; r < 2 * kNB; ++r) sc[r] = p.scale_log2;
+      if (any) softmax_step<kNB, 2, false>(c, a.bits, masked, sc, 1.f, pg, s, pk);
+      // columns that some row sees
+      const uint32_t seen = __reduce_or_sync(0xffffffffu, uint32_t(some));
+      if (nxt.col >= 0) load_aside<kNB>(p, nxt, kvh, qt, mrow, a);
       if (!wait_tile(0x801)) break;
-      if (any) tail_values(smem_u32(ring + at * kTile), pk, seen, g, t, s);
+      if (any) tail_values<kNB>(ring + at * kTile, pk, seen, g, t, s);
     } else {
-      float c[8][4];
-      sealed_scores(smem_u32(ring + at * kTile), sm.q16, g, t, c);
+      float c[kNB][4][4];
+      sealed_scores<kNB>(ring + at * kTile, sm.q16, g, t, c);
       done_tile();
       if (nxt.col >= 0) issue(nxt, true);
-      uint32_t pk[8][2];
-      const float f = p.scale_log2 * a.ks;
-      const float sc[2] = {f * sm.unit[g], f * sm.unit[g + 8]};
-      if (any) softmax_step<8, true>(c, a.bits, masked, sc, a.vs, t, s, pk);
-      if (nxt.col >= 0) load_aside(p, nxt, kvh, qt, mrow, a);
+      uint32_t pk[kNB][4][2];
+      float sc[2 * kNB];
+#pragma unroll
+      for (int r = 0; r < 2 * kNB; ++r) sc[r] = a.ks * q_unit[r];
+      if (any) softmax_step<kNB, 4, true>(c, a.bits, masked, sc, a.vs, pg, s, pk);
+      if (nxt.col >= 0) load_aside<kNB>(p, nxt, kvh, qt, mrow, a);
       if (!wait_tile(0x802)) break;
-      if (any) sealed_values(smem_u32(ring + at * kTile), pk, g, t, s);
+      if (any) sealed_values<kNB>(ring + at * kTile, pk, g, t, s);
     }
     done_tile();
     if (after.col >= 0) issue(after, false);
@@ -596,18 +646,17 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   // ---- join the CTA's warps
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    s.l[r] += __shfl_xor_sync(0xffffffffu, s.l[r], 1);
-    s.l[r] += __shfl_xor_sync(0xffffffffu, s.l[r], 2);
-    if (t == 0) sm.ml[warp][g + 8 * r] = make_float2(s.m[r], s.l[r]);
-    float* dst = reinterpret_cast<float*>(ring) + (g + 8 * r) * (HD + 4);
+  for (int r = 0; r < 2 * kNB; ++r) {
+    const int b = r >> 1, e = r & 1, row = 8 * b + 2 * t + e;
 #pragma unroll
-    for (int e = 0; e < 2; ++e)
+    for (int o = 4; o < 32; o <<= 1) s.l[r] += __shfl_xor_sync(0xffffffffu, s.l[r], o);
+    if (g == 0) sm.ml[warp][row] = make_float2(s.m[r], s.l[r]);
+    float* dst = reinterpret_cast<float*>(ring) + row * (HD + 4) + 16 * pg;
 #pragma unroll
-      for (int i = 0; i < 16; i += 4)
-        *reinterpret_cast<float4*>(dst + 64 * e + 16 * t + i) =
-            make_float4(s.o[i][2 * r + e] * s.unit, s.o[i + 1][2 * r + e] * s.unit,
-                        s.o[i + 2][2 * r + e] * s.unit, s.o[i + 3][2 * r + e] * s.unit);
+    for (int i = 0; i < 8; i += 2)
+      *reinterpret_cast<float4*>(dst + 2 * i) =
+          make_float4(s.o[b][i][e] * s.unit, s.o[b][i][2 + e] * s.unit,
+                      s.o[b][i + 1][e] * s.unit, s.o[b][i + 1][2 + e] * s.unit);
   }
   __syncthreads();
   const size_t tile = size_t(kvh) * gridDim.z + blockIdx.z;
@@ -635,7 +684,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (rec) {
       *reinterpret_cast<float4*>(rec + r * HD + 4 * d4) = acc;
-      if (d4 == 0) reinterpret_cast<float2*>(rec + kRows * HD)[r] = make_float2(m, l);
+      if (d4 == 0) reinterpret_cast<float2*>(rec + kMaxRows * HD)[r] = make_float2(m, l);
     } else if (cluster) {
       // each element is read and written by this thread alone
       *reinterpret_cast<float4*>(reinterpret_cast<float*>(sm.ring[0]) + r * (HD + 4) + 4 * d4) =
@@ -680,8 +729,9 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const Params p, c
   __shared__ float4 acc_s[kJoinWarps][32];
   __shared__ float2 ml_s[kJoinWarps];
   const int row = blockIdx.x, kvh = blockIdx.y, warp = warp_id(), d4 = lane_id();
-  const int r = row % kRows;
-  const float* rec0 = sp.partials + (size_t(kvh) * sp.n_tiles + row / kRows) * sp.splits * kRecord;
+  const int r = row % sp.rows;
+  const float* rec0 =
+      sp.partials + (size_t(kvh) * sp.n_tiles + row / sp.rows) * sp.splits * kRecord;
   float m = -INFINITY, l = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   constexpr int kAt = 8;  // records in flight
@@ -695,7 +745,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const Params p, c
       v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (i < sp.splits) {
         const float* rec = rec0 + size_t(i) * kRecord;
-        x[k] = __ldcg(reinterpret_cast<const float2*>(rec + kRows * HD) + r);
+        x[k] = __ldcg(reinterpret_cast<const float2*>(rec + kMaxRows * HD) + r);
         v[k] = __ldcg(reinterpret_cast<const float4*>(rec + r * HD) + d4);
       }
     }
@@ -753,10 +803,13 @@ using namespace hsd;
 
 namespace {
 constexpr int kMaxDevices = 64;
-std::atomic<bool> g_attr_set[kMaxDevices];
+std::atomic<bool> g_attr_set[2][kMaxDevices];  // [16 rows][device]
 
+// Packed rows of a tile: 8 when they are all, else 16.
+int tile_rows(int q_len, int group) { return int64_t(q_len) * group <= 8 ? 8 : 16; }
 int n_tiles(int q_len, int group) {
-  return int((int64_t(q_len) * group + kv8r::kRows - 1) / kv8r::kRows);
+  const int r = tile_rows(q_len, group);
+  return int((int64_t(q_len) * group + r - 1) / r);
 }
 // CTAs per tile: one wave of one CTA per SM, each warp with a unit at least;
 // up to kMaxCluster of them are a cluster.
@@ -836,6 +889,7 @@ int kv8_rows_launch(const Kv8AttnArgs& a) {
   }
   kv8r::Split sp;
   sp.n_tiles = n_tiles(p.q_len, p.group);
+  sp.rows = tile_rows(p.q_len, p.group);
   sp.splits = n_splits(p.q_len, p.kv_len, p.hq, p.hkv);
   const bool cluster = sp.splits > 1 && sp.splits <= kv8r::kMaxCluster;
   sp.partials = sp.splits > kv8r::kMaxCluster
@@ -853,16 +907,16 @@ int kv8_rows_launch(const Kv8AttnArgs& a) {
     set_error("hsd_verify_attention_kv8: device ordinal %d >= %d", dev, kMaxDevices);
     return HSD_ERR_UNSUPPORTED;
   }
-  if (!g_attr_set[dev].load(std::memory_order_acquire)) {
-    rc = cuda_check(cudaFuncSetAttribute(kv8r::rows_kernel,
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize,
+  const bool wide = sp.rows > 8;
+  const auto kernel = wide ? kv8r::rows_kernel<2> : kv8r::rows_kernel<1>;
+  if (!g_attr_set[wide][dev].load(std::memory_order_acquire)) {
+    rc = cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          int(kv8r::kSmem)),
                     "cudaFuncSetAttribute(rows_kernel)");
     if (rc) return rc;
-    g_attr_set[dev].store(true, std::memory_order_release);
+    g_attr_set[wide][dev].store(true, std::memory_order_release);
   }
-  rc = launch_pdl(kv8r::rows_kernel,
-                  dim3(unsigned(sp.splits), unsigned(p.hkv), unsigned(sp.n_tiles)),
+  rc = launch_pdl(kernel, dim3(unsigned(sp.splits), unsigned(p.hkv), unsigned(sp.n_tiles)),
                   dim3(kv8r::kThreads), kv8r::kSmem, a.stream, "rows_kernel launch",
                   cluster ? unsigned(sp.splits) : 0u, k8, v8, kt, vt, p, sp);
   if (rc || !sp.partials) return rc;
