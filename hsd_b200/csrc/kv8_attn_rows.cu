@@ -125,6 +125,7 @@ __device__ __forceinline__ void bytes_to_f16(uint32_t w, uint32_t& lo, uint32_t&
 struct Walk {
   const uint32_t* list;
   int n_units, stride, u;
+  int room;        // entries that may be read (the list's, or more than it has)
   uint32_t ahead;  // entry of unit u
 };
 struct Step {
@@ -133,7 +134,8 @@ struct Step {
 };
 
 __device__ __forceinline__ uint32_t list_entry(const Walk& w, int u) {
-  return u < w.n_units ? w.list[u >> 1] : 0u;
+  // does not wait for n_units; next_step ignores what lies behind it
+  return (u >> 1) < w.room ? w.list[u >> 1] : 0u;
 }
 
 __device__ __forceinline__ Step next_step(const Params& p, Walk& w, const Step& last) {
@@ -426,18 +428,21 @@ __device__ __forceinline__ void store_row(const Params& p, int kvh, int row, int
 
 // Q rows of the tile in MMA fragment order: MMA 4 h + w covers dims
 // 64 h + 16 t + 4 w..+3 of lane group t; lane 4 g + t has row g of the block.
+// Thread: 8 dims of a row.
+__device__ __forceinline__ uint4 load_q(const Params& p, int kvh, int row0, int n_rows) {
+  const int r = threadIdx.x >> 4, c = threadIdx.x & 15;
+  if (r >= n_rows) return make_uint4(0u, 0u, 0u, 0u);
+  const int i = row0 + r, q = i / p.group;
+  return *reinterpret_cast<const uint4*>(p.q + int64_t(q) * p.q_row_stride +
+                                         int64_t(kvh * p.group + i - q * p.group) *
+                                             p.q_head_stride + 8 * c);
+}
+
 template <int kNB>
-__device__ __forceinline__ void stage_q(const Params& p, Smem& sm, int kvh, int row0, int n_rows) {
+__device__ __forceinline__ void stage_q(Smem& sm, uint4 v) {
   const int tid = threadIdx.x;
   if (tid >= 8 * kNB * 16) return;
-  const int r = tid >> 4, c = tid & 15;  // 8 dims
-  uint4 v = make_uint4(0u, 0u, 0u, 0u);
-  if (r < n_rows) {
-    const int i = row0 + r, q = i / p.group;
-    v = *reinterpret_cast<const uint4*>(p.q + int64_t(q) * p.q_row_stride +
-                                        int64_t(kvh * p.group + i - q * p.group) *
-                                            p.q_head_stride + 8 * c);
-  }
+  const int r = tid >> 4, c = tid & 15;
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
   uint32_t top = 0;
 #pragma unroll
@@ -511,9 +516,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int n_rows = min(kRows, p.q_len * p.group - row0);
   // a tile's rows lie in one query tile: 128 group is a multiple of 16
   const int qt = (row0 / p.group) >> 7;
+  const uint4 q_dims = load_q(p, kvh, row0, n_rows);
   Walk walk;
   walk.list = p.blk_list + size_t(qt) * p.n_kv128;
   walk.n_units = 2 * p.blk_count[qt];
+  walk.room = p.n_kv128;
   walk.stride = sp.splits * kWarps;
   walk.u = int(blockIdx.x) * kWarps + warp;
   walk.ahead = list_entry(walk, walk.u);
@@ -541,12 +548,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   none.col = -1;
   none.tail = none.second = none.partial = false;
   Step cur = next_step(p, walk, none);
-  Step nxt = none;
   if (cur.col >= 0) {
     issue(cur, false);
     issue(cur, true);
-    nxt = next_step(p, walk, cur);
-    if (nxt.col >= 0) issue(nxt, false);
   }
   int mrow[2 * kNB];  // the lane's rows in the query tile, -1: no such row
 #pragma unroll
@@ -556,7 +560,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   Aside<kNB> a;  // of the current step
   if (cur.col >= 0) load_aside<kNB>(p, cur, kvh, qt, mrow, a);
-  stage_q<kNB>(p, sm, kvh, row0, n_rows);
+  stage_q<kNB>(sm, q_dims);
+  Step nxt = none;
+  if (cur.col >= 0) nxt = next_step(p, walk, cur);
+  if (nxt.col >= 0) issue(nxt, false);
   __syncthreads();  // Q fragments and the abort word
 
   State<kNB> s;
