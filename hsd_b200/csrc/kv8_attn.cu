@@ -136,8 +136,19 @@ ManyLayout many_layout(int32_t kv_len, int32_t hkv) {
   return m;
 }
 
-// Rows kernel or many rows.
-bool use_rows(int32_t q_len, int32_t group) { return int64_t(q_len) * group <= 256; }
+// Rows kernel or many rows, by the time each takes.  Many rows: 40 us however
+// small (items cut between all SMs and joined by their first CTA one after
+// another), the expansion (1.3e-4 us a column and KV head), and 2.4 us per SM for
+// every 128 rows x 128 columns x two heads.  Measured (rows / many, us): 12/2
+// heads, 1600 columns: 128 rows 18 / 42, 256 rows 34 / 40, 384 rows 36 / 35; 8192
+// columns: 32 rows 32 / 63, 128 rows 58 / 62, 256 rows 112 / 53; 16/8 heads, 32768
+// columns: 32 rows 61 / 115, 128 rows 207 / 113.
+bool use_rows(int32_t q_len, int32_t kv_len, int32_t hq, int32_t hkv) {
+  const float tiles = float((q_len + 127) / 128) * float((hq / hkv + 1) / 2) * float(hkv);
+  const float many = 40.f + 1.3e-4f * float(kv_len) * float(hkv) +
+                     tiles * float((kv_len + 127) / 128) * (2.4f / 148.f);
+  return hsd_host::kv8_rows_us(q_len, kv_len, hq, hkv) <= many;
+}
 
 int many_launch(const hsd_host::Kv8AttnArgs& a, const hsd_plan_t& plan, float scale) {
   using namespace hsd;
@@ -216,7 +227,7 @@ extern "C" size_t hsd_kv8_attention_workspace_bytes(int32_t q_len, int32_t kv_le
   if (q_len <= 0 || kv_len <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 ||
       num_q_heads % num_kv_heads)
     return 0;
-  if (use_rows(q_len, num_q_heads / num_kv_heads))
+  if (use_rows(q_len, kv_len, num_q_heads, num_kv_heads))
     return hsd_host::kv8_rows_workspace_bytes(q_len, kv_len, num_q_heads, num_kv_heads);
   return many_layout(kv_len, num_kv_heads).total;
 }
@@ -304,5 +315,6 @@ extern "C" int hsd_verify_attention_kv8(
   a.vt_head_stride = vt_head_stride;
   a.workspace = workspace;
   a.stream = reinterpret_cast<cudaStream_t>(stream);
-  return use_rows(q_len, p.group) ? hsd_host::kv8_rows_launch(a) : many_launch(a, *plan, scale);
+  return use_rows(q_len, kv_len, num_q_heads, num_kv_heads) ? hsd_host::kv8_rows_launch(a)
+                                                             : many_launch(a, *plan, scale);
 }

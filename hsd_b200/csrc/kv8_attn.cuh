@@ -58,6 +58,8 @@ struct Kv8AttnArgs {
   void* workspace;
   cudaStream_t stream;
 };
+// What the rows kernel takes for these sizes, by its own model.
+float kv8_rows_us(int q_len, int kv_len, int hq, int hkv);
 size_t kv8_rows_workspace_bytes(int q_len, int kv_len, int hq, int hkv);
 int kv8_rows_launch(const Kv8AttnArgs& a);
 // 3-D map {128 dims, rows, heads} of int8 (box 128 x box_rows) or bf16 (box

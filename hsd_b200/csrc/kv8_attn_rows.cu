@@ -41,6 +41,7 @@
 
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <atomic>
 
 namespace hsd {
@@ -812,25 +813,91 @@ namespace {
 constexpr int kMaxDevices = 64;
 std::atomic<bool> g_attr_set[2][kMaxDevices];  // [16 rows][device]
 
+auto rows_kernel_of(bool wide) { return wide ? kv8r::rows_kernel<2> : kv8r::rows_kernel<1>; }
+
+int set_rows_attribute(bool wide, int dev) {
+  if (g_attr_set[wide][dev].load(std::memory_order_acquire)) return HSD_OK;
+  const int rc = cuda_check(
+      cudaFuncSetAttribute(rows_kernel_of(wide), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           int(kv8r::kSmem)),
+      "cudaFuncSetAttribute(rows_kernel)");
+  if (rc == HSD_OK) g_attr_set[wide][dev].store(true, std::memory_order_release);
+  return rc;
+}
+
 // Packed rows of a tile: 8 when they are all, else 16.
 int tile_rows(int q_len, int group) { return int64_t(q_len) * group <= 8 ? 8 : 16; }
 int n_tiles(int q_len, int group) {
   const int r = tile_rows(q_len, group);
   return int((int64_t(q_len) * group + r - 1) / r);
 }
-// CTAs per tile: one wave of one CTA per SM, each warp with a unit at least;
-// up to kMaxCluster of them are a cluster.
-int n_splits(int q_len, int kv_len, int hq, int hkv) {
+std::atomic<int> g_clusters[2][kMaxDevices][kv8r::kMaxCluster + 1];
+
+// Clusters of s CTAs that the current device runs at once (SMs of a cluster lie
+// in one group of the chip, so this is less than SMs / s).
+int resident_clusters(bool wide, int s) {
+  const int sms = kv8_sm_count();
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return sms / s;
+  int n = g_clusters[wide][dev][s].load(std::memory_order_relaxed);
+  if (n > 0) return n;
+  n = sms / s;
+  if (s > 1 && set_rows_attribute(wide, dev) == HSD_OK) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned(s * sms));
+    cfg.blockDim = dim3(kv8r::kThreads);
+    cfg.dynamicSmemBytes = kv8r::kSmem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = unsigned(s);
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int m = 0;
+    if (cudaOccupancyMaxActiveClusters(&m, rows_kernel_of(wide), &cfg) == cudaSuccess && m > 0)
+      n = m;
+  }
+  if (cudaGetLastError() == cudaSuccess) g_clusters[wide][dev][s].store(n);
+  return n;
+}
+
+// CTAs per tile and what the launch then takes.  With every SM busy a warp's step
+// takes about 3.3 us (16 rows; 2 us for 8) and a CTA 5 us besides (measured at 1600
+// to 32768 columns), so the time goes by the waves of clusters and the steps of a
+// warp; more than kMaxCluster CTAs per tile, when there are few tiles, need the
+// join kernel (4 us).
+struct Choice {
+  int splits;
+  float us;
+};
+Choice choose(int q_len, int kv_len, int hq, int hkv) {
   const int64_t tiles = int64_t(n_tiles(q_len, hq / hkv)) * hkv;
+  const bool wide = tile_rows(q_len, hq / hkv) > 8;
   const int units = (kv_len + 63) / 64;
   const int most = (units + kv8r::kWarps - 1) / kv8r::kWarps;
-  const int64_t s = kv8_sm_count() / tiles;
-  return s < 1 ? 1 : s > most ? most : int(s);
+  auto time = [&](int64_t waves, int s) {
+    const int steps = (units + s * kv8r::kWarps - 1) / (s * kv8r::kWarps);
+    return float(waves) * (5.f + (wide ? 3.3f : 2.f) * float(steps));
+  };
+  Choice best{1, time((tiles + kv8_sm_count() - 1) / kv8_sm_count(), 1)};
+  for (int s = 2; s <= kv8r::kMaxCluster && s <= most; ++s) {
+    const int at_once = resident_clusters(wide, s);
+    const float us = time((tiles + at_once - 1) / at_once, s);
+    if (us < best.us) best = {s, us};
+  }
+  const int64_t s = std::min<int64_t>(kv8_sm_count() / tiles, most);
+  if (s > kv8r::kMaxCluster && time(1, int(s)) + 4.f < best.us)
+    best = {int(s), time(1, int(s)) + 4.f};
+  return best;
 }
 }  // namespace
 
+float kv8_rows_us(int q_len, int kv_len, int hq, int hkv) {
+  return choose(q_len, kv_len, hq, hkv).us;
+}
+
 size_t kv8_rows_workspace_bytes(int q_len, int kv_len, int hq, int hkv) {
-  const int s = n_splits(q_len, kv_len, hq, hkv);
+  const int s = choose(q_len, kv_len, hq, hkv).splits;
   if (s <= kv8r::kMaxCluster) return kKv8FlagBytes;
   return kKv8FlagBytes + size_t(n_tiles(q_len, hq / hkv)) * hkv * s * kv8r::kRecord * sizeof(float);
 }
@@ -897,7 +964,7 @@ int kv8_rows_launch(const Kv8AttnArgs& a) {
   kv8r::Split sp;
   sp.n_tiles = n_tiles(p.q_len, p.group);
   sp.rows = tile_rows(p.q_len, p.group);
-  sp.splits = n_splits(p.q_len, p.kv_len, p.hq, p.hkv);
+  sp.splits = choose(p.q_len, p.kv_len, p.hq, p.hkv).splits;
   const bool cluster = sp.splits > 1 && sp.splits <= kv8r::kMaxCluster;
   sp.partials = sp.splits > kv8r::kMaxCluster
                     ? reinterpret_cast<float*>(static_cast<char*>(a.workspace) + kKv8FlagBytes)
@@ -915,15 +982,9 @@ int kv8_rows_launch(const Kv8AttnArgs& a) {
     return HSD_ERR_UNSUPPORTED;
   }
   const bool wide = sp.rows > 8;
-  const auto kernel = wide ? kv8r::rows_kernel<2> : kv8r::rows_kernel<1>;
-  if (!g_attr_set[wide][dev].load(std::memory_order_acquire)) {
-    rc = cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         int(kv8r::kSmem)),
-                    "cudaFuncSetAttribute(rows_kernel)");
-    if (rc) return rc;
-    g_attr_set[wide][dev].store(true, std::memory_order_release);
-  }
-  rc = launch_pdl(kernel, dim3(unsigned(sp.splits), unsigned(p.hkv), unsigned(sp.n_tiles)),
+  rc = set_rows_attribute(wide, dev);
+  if (rc) return rc;
+  rc = launch_pdl(rows_kernel_of(wide), dim3(unsigned(sp.splits), unsigned(p.hkv), unsigned(sp.n_tiles)),
                   dim3(kv8r::kThreads), kv8r::kSmem, a.stream, "rows_kernel launch",
                   cluster ? unsigned(sp.splits) : 0u, k8, v8, kt, vt, p, sp);
   if (rc || !sp.partials) return rc;
