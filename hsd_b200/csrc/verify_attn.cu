@@ -94,10 +94,11 @@ struct __align__(1024) Smem {
   uint8_t pb[NSLOT][TILE_BYTES];  // P of the current block per slot (MMA A operand)
   uint8_t kv[NSTAGE][TILE_BYTES];
   // kScaled: the scales of a block's halves, four blocks in turn, copied with
-  // its K tile.  Block n + 3's K tile is loaded after PV(n), hence after the
-  // softmax of block n.
+  // its K tile and counted on that tile's barrier; the MMA issuers wait for it
+  // and arrive on bar_s_full themselves too, which hands the scales on to the
+  // softmax (a barrier of their own for it cost 4 %).  Block n + 3's K tile is
+  // loaded after PV(n), hence after the softmax of block n.
   ColumnScale scales[NSCALE][2];
-  uint64_t bar_scales[NSCALE];
   uint64_t bar_q;
   uint64_t bar_q_free;
   uint64_t bar_full[NSTAGE];
@@ -215,6 +216,12 @@ __device__ __forceinline__ int range_start(int k, int total, int g) {
 constexpr uint32_t kIdescS = idesc_bf16_f32(BM, BN, false, false);  // Q K^T: both K-major
 constexpr uint32_t kIdescO = idesc_bf16_f32(BM, HD, false, true);   // P V: V is MN-major
 
+__device__ __forceinline__ float sum4(uint64_t a, uint64_t b) {
+  float s0, s1, s2, s3;
+  f2_unpack(a, s0, s1);
+  f2_unpack(b, s2, s3);
+  return (s0 + s1) + (s2 + s3);
+}
 __device__ __forceinline__ float sum8(const uint64_t (&s)[4]) {
   float s0, s1, s2, s3, s4, s5, s6, s7;
   f2_unpack(s[0], s0, s1);
@@ -272,10 +279,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&sm.bar_full[i], 1);
       mbar_init(&sm.bar_empty[i], NSLOT);
     }
-    if constexpr (kScaled)
-      for (int i = 0; i < NSCALE; ++i) mbar_init(&sm.bar_scales[i], 1);
     for (int i = 0; i < NSLOT; ++i) {
-      mbar_init(&sm.bar_s_full[i], 1);
+      mbar_init(&sm.bar_s_full[i], kScaled ? 2 : 1);
       mbar_init(&sm.bar_s_free[i], 128);
       mbar_init(&sm.bar_p_full[i], 128);
       mbar_init(&sm.bar_o_done[i], 1);
@@ -357,17 +362,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int kb = int(list[j] & 0xFFFFFFu);
           ok = mbar_wait(&sm.bar_empty[stage], phase ^ 1u, abort, p.status, 0x100 + int(is_v));
           if (!ok) break;
-          if constexpr (kScaled) {
-            if (!is_v) {
-              uint64_t* bar = &sm.bar_scales[blocks & (NSCALE - 1)];
-              mbar_arrive_expect_tx(bar, 2 * sizeof(ColumnScale));
-              bulk_load(sm.scales[blocks & (NSCALE - 1)],
-                        p.col_scale + size_t(pc.kvh) * (2 * p.n_kv128) + 2 * kb,
-                        2 * sizeof(ColumnScale), bar);
-              ++blocks;
-            }
+          const bool with_scales = kScaled && !is_v;
+          mbar_arrive_expect_tx(&sm.bar_full[stage],
+                                TILE_BYTES + (with_scales ? 2 * sizeof(ColumnScale) : 0));
+          if (with_scales) {
+            bulk_load(sm.scales[blocks & (NSCALE - 1)],
+                      p.col_scale + size_t(pc.kvh) * (2 * p.n_kv128) + 2 * kb,
+                      2 * sizeof(ColumnScale), &sm.bar_full[stage]);
+            ++blocks;
           }
-          mbar_arrive_expect_tx(&sm.bar_full[stage], TILE_BYTES);
           const CUtensorMap* tm = is_v ? &tm_v : &tm_k;
           for (int d = 0; d < 2; ++d)
             tma_load_3d(sm.kv[stage] + d * SUB_BYTES, tm, &sm.bar_full[stage], d * 64, kb * BN,
@@ -389,10 +392,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (pieces > 0)
         mbar_wait(&sm.bar_q, uint32_t(pieces - 1) & 1u, abort, p.status, 0x120, false);
-      if constexpr (kScaled)
-        for (int i = 0; i < min(blocks, NSCALE); ++i)
-          mbar_wait(&sm.bar_scales[i], uint32_t((blocks - 1 - i) / NSCALE) & 1u, abort, p.status,
-                    0x130 + i, false);
     } else if ((warp == 9 || warp == 11) && lane == 0) {
       // ---------------------------------------------------------- MMA issuers
       // One thread per slot (warp 9: slot 0, warp 11: slot 1), so each slot's
@@ -449,6 +448,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_fence_after();
             issue_s(t_sl, qa, kv0 + st * TILE_BYTES);
             umma_commit(&sm.bar_s_full[s]);
+            if constexpr (kScaled) mbar_arrive(&sm.bar_s_full[s]);  // hands the scales on
             ++ns;
             // the piece's last S: Q is free once it completes, so the next
             // piece's Q loads under this block's softmax and PV
@@ -564,13 +564,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                           uint32_t(wd_next[1] >> 32)};
         if (j + 1 < pc.b1) e_next = list[j + 1];
         const ColumnScale* sc = sm.scales[nb & (NSCALE - 1)];
-        if constexpr (kScaled) {
-          ok = __all_sync(0xffffffffu,
-                          mbar_wait(&sm.bar_scales[nb & (NSCALE - 1)], uint32_t(nb / NSCALE) & 1u,
-                                    abort, p.status, 0x302 + s));
-          if (!ok) break;
-          ++nb;
-        }
+        if constexpr (kScaled) ++nb;
         ok = __all_sync(0xffffffffu, mbar_wait(&sm.bar_s_full[s], uint32_t(gs) & 1u, abort,
                                                p.status, 0x300 + s));
         if (!ok) break;
@@ -688,7 +682,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         // subtract and row sums run on packed fp32 pairs.
         uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2);
         uint64_t nm2 = f2_pack(nm, nm);
-        float half_sum = 0.f;  // kScaled: the first half's row sum
         uint64_t sum2[4] = {0ull, 0ull, 0ull, 0ull};
         const uint32_t prow = smem_u32(sm.pb[s]) + uint32_t(r) * 128u;
 #pragma unroll
@@ -696,11 +689,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           if constexpr (kScaled) {
             sc2 = f2_pack(sc[c].score, sc[c].score);
             nm2 = f2_pack(nm + sc[c].log2_v, nm + sc[c].log2_v);
-            if (c == 1) {
-              half_sum = sum8(sum2) * sc[0].inv_v;
-#pragma unroll
-              for (int i = 0; i < 4; ++i) sum2[i] = 0ull;
-            }
           }
 #pragma unroll
           for (int ch = 0; ch < 8; ++ch) {
@@ -712,7 +700,9 @@ __global__ void __launch_bounds__(kThreads, 1)
               f2_unpack(f2_fma(f2_pack(x[col], x[col + 1]), sc2, nm2), xa, xb);
               const float a = ex2_approx(xa);
               const float b = ex2_approx(xb);
-              sum2[i] = f2_add(sum2[i], f2_pack(a, b));
+              // kScaled: two sums per half, else four
+              const int k = kScaled ? 2 * c + (i & 1) : i;
+              sum2[k] = f2_add(sum2[k], f2_pack(a, b));
               pk[i] = pack_bf16x2_trunc(a, b);
             }
             st_shared_v4(prow + uint32_t(c * SUB_BYTES) + (uint32_t(ch ^ (r & 7)) << 4), pk[0],
@@ -724,7 +714,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           ++hs;
         }
         if constexpr (kScaled)
-          l = l * alpha + (half_sum + sum8(sum2) * sc[1].inv_v) * kPackBiasInv;
+          l = l * alpha +
+              (sum4(sum2[0], sum2[1]) * sc[0].inv_v + sum4(sum2[2], sum2[3]) * sc[1].inv_v) *
+                  kPackBiasInv;
         else
           l = l * alpha + sum8(sum2) * kPackBiasInv;
         tmem_wait_st();  // O rescale stores, if any
