@@ -4,13 +4,17 @@
 // Many rows.  Every K and V element meets every query tile and head pair (17 x
 // 3 times for a region page), so converting where it is used costs far more
 // than the cache's bytes; here one launch expands the layer's columns into
-// the workspace -- int8 to the same integers in bf16, exactly, the bf16 tail
-// copied behind them -- and the tcgen05 verification kernel (verify_attn.cu)
-// reads that, with one score factor and one V factor per 64 columns in its
-// softmax.  The expansion is bound by HBM and L2: 1 byte read and 2 written per
-// sealed value, and the attention finds it in L2.
+// the workspace and the tcgen05 verification kernel (verify_attn.cu) reads that,
+// with one score factor and one V factor per 64 columns in its softmax.  K
+// becomes bf16 (int8: the same integers, exactly; the bf16 tail copied), V fp16
+// (int8 exactly; 64 tail rows times the power of two that brings their largest
+// value to [64, 128): exact down to 2^-21 of it, else within 2^-31 of it), so that
+// P can be fp16 and keep 11 bits.  The expansion is bound by HBM and L2: 1 byte
+// read and 2 written per sealed value, and the attention finds it in L2.
 #include "kv8_attn.cuh"
 #include "verify_attn.cuh"
+
+#include <cuda_fp16.h>
 
 namespace hsd {
 namespace kv8a {
@@ -24,13 +28,14 @@ struct ExpandParams {
   int64_t row_stride[2], head_stride[2];
   const uint8_t* tile_class;
   const uint64_t* mask_words;
-  __nv_bfloat16* dst;  // [2][hkv][kv_len][128]
+  uint16_t* dst;  // [2][hkv][kv_len][128]: K bf16, V fp16
   attn::ColumnScale* col_scale;
   int kv_len, hkv, n_kv64, n_qtiles, sealed, tail_row0;
   float scale_log2;
 };
 
 constexpr int kExpandThreads = 256;
+constexpr float kMinVScale = 8.077935669463161e-28f;  // 2^-90
 
 // Columns of a 64-column tile that some query row sees.
 __device__ __forceinline__ uint64_t seen_columns(const ExpandParams& p, int t, uint32_t* red) {
@@ -56,24 +61,46 @@ __device__ __forceinline__ uint64_t seen_columns(const ExpandParams& p, int t, u
 // CTA (64-column tile, KV head, K or V)
 __global__ void __launch_bounds__(kExpandThreads) expand_kernel(const ExpandParams p) {
   pdl_wait_then_release();  // launched with launch_pdl
-  __shared__ uint32_t red[2];
+  __shared__ uint32_t red[2], warp_top[kExpandThreads / 32];
   const int t = blockIdx.x, h = blockIdx.y, z = blockIdx.z, tid = threadIdx.x;
   const int col0 = 64 * t;
   uint4* dst = reinterpret_cast<uint4*>(
       p.dst + (size_t(z * p.hkv + h) * p.kv_len + col0) * HD);
+  float v_unit = 1.f;  // V: value = fp16 * v_unit
   if (col0 < p.sealed) {
     const uint4* src =
         reinterpret_cast<const uint4*>(p.x8[z] + h * p.head_stride8[z] + int64_t(col0) * HD);
     uint4 v[2];
     v[0] = __ldcs(src + tid);
     v[1] = __ldcs(src + tid + kExpandThreads);
+    // A block of next to nothing (zeros are sealed with the scale 2^-100 / 127)
+    // takes the scale 2^-90, so that its columns' part of the row sum, formed as
+    // P / scale, does not underflow.
+    float tiny = 0.f;
+    if (z == 1) {
+      const float vs = p.scale[1][h * p.scale_stride + t];
+      v_unit = fmaxf(vs, kMinVScale);
+      if (vs < kMinVScale) tiny = vs / kMinVScale;
+    }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       uint32_t o[8];
-      bytes_to_bf16(v[u].x, o[0], o[1]);
-      bytes_to_bf16(v[u].y, o[2], o[3]);
-      bytes_to_bf16(v[u].z, o[4], o[5]);
-      bytes_to_bf16(v[u].w, o[6], o[7]);
+      const uint32_t in[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (z == 0) {
+          bytes_to_bf16(in[i], o[2 * i], o[2 * i + 1]);
+        } else {
+          bytes_to_f16(in[i], o[2 * i], o[2 * i + 1]);
+          if (tiny > 0.f) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&o[2 * i + k]));
+              o[2 * i + k] = pack_f16x2(x.x * tiny, x.y * tiny);
+            }
+          }
+        }
+      }
       const int at = 2 * (tid + u * kExpandThreads);
       dst[at] = make_uint4(o[0], o[1], o[2], o[3]);
       dst[at + 1] = make_uint4(o[4], o[5], o[6], o[7]);
@@ -92,27 +119,55 @@ __global__ void __launch_bounds__(kExpandThreads) expand_kernel(const ExpandPara
       if (r < rows && ((seen >> r) & 1ull))
         v[u] = __ldg(reinterpret_cast<const uint4*>(src + r * p.row_stride[z]));
     }
+    if (z == 1) {
+      // the block's largest finite magnitude, as bf16 bits
+      uint32_t top = 0;
+      const uint32_t* w = &v[0].x;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const uint32_t lo = w[i] & 0x7FFFu, hi = (w[i] >> 16) & 0x7FFFu;
+        top = max(top, max(lo < 0x7F80u ? lo : 0u, hi < 0x7F80u ? hi : 0u));
+      }
+      top = __reduce_max_sync(0xffffffffu, top);
+      if (lane_id() == 0) warp_top[warp_id()] = top;
+      __syncthreads();
+      top = __reduce_max_sync(0xffffffffu, warp_top[lane_id() & (kExpandThreads / 32 - 1)]);
+      // v_unit = 2^(e - 6) for a largest value in [2^e, 2^(e + 1)); e as a float's
+      // exponent field, held where both v_unit and its inverse are normal
+      const uint32_t e = top == 0u ? 133u : min(max(top >> 7, 40u), 250u);
+      v_unit = __uint_as_float((e - 6u) << 23);
+      const float inv = __uint_as_float((260u - e) << 23);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        uint32_t* x = &v[u].x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          x[i] = pack_f16x2(__uint_as_float(x[i] << 16) * inv,
+                            __uint_as_float(x[i] & 0xFFFF0000u) * inv);
+      }
+    }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int r = 16 * u + (tid >> 4);
       if (r < rows) dst[r * 16 + (tid & 15)] = v[u];
     }
   }
-  if (z == 0 && tid == 0) {
-    float ks = 1.f, vs = 1.f;
-    if (col0 < p.sealed) {
-      ks = p.scale[0][h * p.scale_stride + t];
-      vs = p.scale[1][h * p.scale_stride + t];
-    }
-    attn::ColumnScale c;
-    c.score = ks * p.scale_log2;
-    c.log2_v = log2f(vs);
-    c.inv_v = 1.f / vs;
-    c.pad = 0.f;
-    attn::ColumnScale* dst_scale = p.col_scale + size_t(h) * ((p.n_kv64 + 1) & ~1) + t;
-    dst_scale[0] = c;
+  // score factor by the K CTA, V factors by the V CTA
+  if (tid == 0) {
+    attn::ColumnScale* c = p.col_scale + size_t(h) * ((p.n_kv64 + 1) & ~1) + t;
     // the absent second half of an odd last block: any finite factors
-    if (t == p.n_kv64 - 1 && (t & 1) == 0) dst_scale[1] = {1.f, 0.f, 1.f, 0.f};
+    const bool pad = t == p.n_kv64 - 1 && (t & 1) == 0;
+    if (z == 0) {
+      c->score = (col0 < p.sealed ? p.scale[0][h * p.scale_stride + t] : 1.f) * p.scale_log2;
+      if (pad) c[1].score = 1.f;
+    } else {
+      c->log2_v = log2f(v_unit);
+      c->inv_v = 1.f / v_unit;
+      if (pad) {
+        c[1].log2_v = 0.f;
+        c[1].inv_v = 1.f;
+      }
+    }
   }
 }
 
@@ -177,7 +232,7 @@ int many_launch(const hsd_host::Kv8AttnArgs& a, const hsd_plan_t& plan, float sc
   e.head_stride[1] = a.vt_head_stride;
   e.tile_class = plan.tile_class;
   e.mask_words = plan.mask_words;
-  e.dst = reinterpret_cast<__nv_bfloat16*>(ws + m.rows);
+  e.dst = reinterpret_cast<uint16_t*>(ws + m.rows);
   e.col_scale = reinterpret_cast<attn::ColumnScale*>(ws + m.scales);
   e.kv_len = p.kv_len;
   e.hkv = p.hkv;

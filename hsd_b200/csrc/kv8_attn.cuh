@@ -39,6 +39,27 @@ __device__ __forceinline__ void bytes_to_bf16(uint32_t w, uint32_t& lo, uint32_t
   asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(hi) : "r"(p1 & 0xFF7FFF7Fu), "r"(p1 & 0xFF80FF80u));
 }
 
+// Bytes `sel` (two nibble pairs) of a word of n + 128 -> two exact fp16: 1024 +
+// 128 + n is the byte under the exponent of 1024.
+__device__ __forceinline__ uint32_t biased_to_f16(uint32_t w, uint32_t sel) {
+  uint32_t r;
+  const uint32_t p = __byte_perm(w, 0x64646464u, sel);
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(p), "r"(0x64806480u));
+  return r;
+}
+// Four signed bytes -> two fp16 pairs, exactly.
+__device__ __forceinline__ void bytes_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  const uint32_t b = w ^ 0x80808080u;
+  lo = biased_to_f16(b, 0x4140);
+  hi = biased_to_f16(b, 0x4342);
+}
+
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
 }  // namespace kv8a
 }  // namespace hsd
 

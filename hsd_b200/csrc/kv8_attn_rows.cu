@@ -39,8 +39,6 @@
 // and no flags: the result does not depend on the order in which CTAs finish.
 #include "kv8_attn.cuh"
 
-#include <cuda_fp16.h>
-
 #include <algorithm>
 #include <atomic>
 
@@ -48,6 +46,9 @@ namespace hsd {
 namespace kv8r {
 
 using kv8a::HD;
+using kv8a::biased_to_f16;
+using kv8a::bytes_to_f16;
+using kv8a::pack_f16x2;
 using kv8a::Params;
 
 constexpr int kWarps = 8;
@@ -99,26 +100,6 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
 
 __device__ __forceinline__ uint4 lds128(const uint8_t* p) {
   return *reinterpret_cast<const uint4*>(p);
-}
-
-__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-
-// Bytes `sel` (two nibble pairs) of a word of n + 128 -> two exact fp16.
-__device__ __forceinline__ uint32_t biased_to_f16(uint32_t w, uint32_t sel) {
-  uint32_t r;
-  const uint32_t p = __byte_perm(w, 0x64646464u, sel);
-  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(p), "r"(0x64806480u));  // 1152
-  return r;
-}
-// Four signed bytes -> two fp16 pairs.
-__device__ __forceinline__ void bytes_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  const uint32_t b = w ^ 0x80808080u;
-  lo = biased_to_f16(b, 0x4140);
-  hi = biased_to_f16(b, 0x4342);
 }
 
 // The warp's walk over its units: 64-column halves of the tile's block list,
@@ -370,7 +351,8 @@ __device__ __forceinline__ void tail_scores(const uint8_t* kb, const uint2 (*qbf
     for (int cc = 0; cc < 2; ++cc)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const uint8_t* row = kb + h * (kTile / 2) + (16 * j + pg) * 128 + (((2 * t + cc) ^ pg) << 4);
+        const uint8_t* row =
+            kb + h * (kTile / 2) + (16 * j + pg) * 128 + (((2 * t + cc) ^ pg) << 4);
         const uint4 x = lds128(row), y = lds128(row + 8 * 128);
         const uint32_t a0[4] = {x.x, y.x, x.y, y.y}, a1[4] = {x.z, y.z, x.w, y.w};
 #pragma unroll
@@ -497,9 +479,10 @@ __device__ __forceinline__ void cluster_sync() {
 // CTA (split, KV head, tile of 8 kNB packed rows)
 template <int kNB>
 __global__ void __launch_bounds__(kThreads, 1)
-    rows_kernel(const __grid_constant__ CUtensorMap tm_k8, const __grid_constant__ CUtensorMap tm_v8,
-                const __grid_constant__ CUtensorMap tm_kt, const __grid_constant__ CUtensorMap tm_vt,
-                const Params p, const Split sp) {
+    rows_kernel(const __grid_constant__ CUtensorMap tm_k8,
+                const __grid_constant__ CUtensorMap tm_v8,
+                const __grid_constant__ CUtensorMap tm_kt,
+                const __grid_constant__ CUtensorMap tm_vt, const Params p, const Split sp) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
   // (offset from the array, so that the compiler knows these are shared loads)
   Smem& sm = *reinterpret_cast<Smem*>(smem_raw + ((0u - smem_u32(smem_raw)) & 1023u));
@@ -984,7 +967,8 @@ int kv8_rows_launch(const Kv8AttnArgs& a) {
   const bool wide = sp.rows > 8;
   rc = set_rows_attribute(wide, dev);
   if (rc) return rc;
-  rc = launch_pdl(rows_kernel_of(wide), dim3(unsigned(sp.splits), unsigned(p.hkv), unsigned(sp.n_tiles)),
+  rc = launch_pdl(rows_kernel_of(wide),
+                  dim3(unsigned(sp.splits), unsigned(p.hkv), unsigned(sp.n_tiles)),
                   dim3(kv8r::kThreads), kv8r::kSmem, a.stream, "rows_kernel launch",
                   cluster ? unsigned(sp.splits) : 0u, k8, v8, kt, vt, p, sp);
   if (rc || !sp.partials) return rc;

@@ -514,8 +514,9 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return nullptr;
 }
 
-#define HSD_METHOD(f) \
-  {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&entry<f>)), METH_FASTCALL, nullptr}
+#define HSD_METHOD(f)                                                                  \
+  {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&entry<f>)), METH_FASTCALL, \
+   nullptr}
 PyMethodDef kMethods[] = {HSD_METHOD(rope_append_axes), HSD_METHOD(kv8_seal),
                           HSD_METHOD(kv8_unseal), HSD_METHOD(verify_attention_kv8),
                           {nullptr, nullptr, 0, nullptr}};

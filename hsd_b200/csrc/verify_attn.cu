@@ -49,9 +49,12 @@
 // kScaled (the attention over the 8-bit cache, kv8_attn.cu): every 64 columns
 // have a K scale, which multiplies their scores, and a V scale, which enters
 // the exponent as its logarithm and is divided out of their part of the row
-// sum, so P carries it at no cost per element.  The partial records hold fp16
-// with a power of two per row there (2^-12 of the row's largest value): bf16
-// records add as much error as P's own rounding.
+// sum, so P carries it at no cost per element.  The running maximum is that of
+// score + log2(V scale), so P always is at most 2^8 times 2^kPShift, and P and V
+// are fp16 (V's values are int8, or bf16 times a power of two): P keeps 11 bits,
+// and rounding it to nearest is as fast as truncating to bf16.  The partial
+// records hold fp16 with a power of two per row (2^-12 of the row's largest
+// value).
 #include <atomic>
 
 #include "common.cuh"
@@ -214,7 +217,10 @@ __device__ __forceinline__ int range_start(int k, int total, int g) {
 }
 
 constexpr uint32_t kIdescS = idesc_bf16_f32(BM, BN, false, false);  // Q K^T: both K-major
-constexpr uint32_t kIdescO = idesc_bf16_f32(BM, HD, false, true);   // P V: V is MN-major
+template <bool kScaled>  // P V: V is MN-major
+constexpr uint32_t kIdescO =
+    kScaled ? idesc_f16_f32(BM, HD, false, true) : idesc_bf16_f32(BM, HD, false, true);
+constexpr float kPShift = 7.0f;  // kScaled: log2 of the factor on P; 2^(8 + 7) < 65504
 
 __device__ __forceinline__ float sum4(uint64_t a, uint64_t b) {
   float s0, s1, s2, s3;
@@ -246,6 +252,7 @@ __device__ __forceinline__ void issue_s(uint32_t d_tmem, uint32_t q_smem, uint32
 
 // O (+)= P V: P K-major in smem (the layout of Q), V MN-major in smem;
 // K step = 16 KV rows.
+template <bool kScaled>
 __device__ __forceinline__ void issue_pv(uint32_t d_tmem, uint32_t p_smem, uint32_t v_smem,
                                          bool acc) {
   const uint64_t a = sdesc_sw128(p_smem, 16, 1024);
@@ -253,7 +260,7 @@ __device__ __forceinline__ void issue_pv(uint32_t d_tmem, uint32_t p_smem, uint3
 #pragma unroll
   for (int kk = 0; kk < BN / 16; ++kk) {
     const uint64_t a_off = uint64_t(((kk >> 2) * SUB_BYTES + (kk & 3) * 32) >> 4);
-    umma_bf16_ss(d_tmem, a + a_off, b + uint64_t((kk * 2048) >> 4), kIdescO,
+    umma_bf16_ss(d_tmem, a + a_off, b + uint64_t((kk * 2048) >> 4), kIdescO<kScaled>,
                  (acc || kk > 0) ? 1u : 0u);
   }
 }
@@ -464,7 +471,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (!ok) break;
             }
             tc_fence_after();
-            issue_pv(t_sl + 128, pa, kv0 + st * TILE_BYTES, j > pc.b0);
+            issue_pv<kScaled>(t_sl + 128, pa, kv0 + st * TILE_BYTES, j > pc.b0);
             umma_commit(&sm.bar_o_done[s]);
             ++gs;
           }
@@ -592,7 +599,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         float m_new;
         if constexpr (kScaled) {
-          // per half: four independent chains, then the half's scale
+          // per half: four independent chains, then the half's scales
           float mx4[2][4];
 #pragma unroll
           for (int hf = 0; hf < 2; ++hf) {
@@ -604,9 +611,12 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int k = 0; k < 4; ++k)
                 mx4[hf][k] = fmax3(mx4[hf][k], x[64 * hf + i + k], x[64 * hf + i + 4 + k]);
           }
-          m_new = fmax3(m,
-                        fmaxf(fmax3(mx4[0][0], mx4[0][1], mx4[0][2]), mx4[0][3]) * sc[0].score,
-                        fmaxf(fmax3(mx4[1][0], mx4[1][1], mx4[1][2]), mx4[1][3]) * sc[1].score);
+          m_new = fmax3(
+              m,
+              fmaf(fmaxf(fmax3(mx4[0][0], mx4[0][1], mx4[0][2]), mx4[0][3]), sc[0].score,
+                   sc[0].log2_v),
+              fmaf(fmaxf(fmax3(mx4[1][0], mx4[1][1], mx4[1][2]), mx4[1][3]), sc[1].score,
+                   sc[1].log2_v));
         } else {
           // row max: eight independent chains, then a tree
           float mx8[8];
@@ -625,7 +635,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool need = m_new > m + kRescaleLog2;  // also true for m = -inf, m_new finite
         const float alpha = need ? ex2_approx(m - m_new) : 1.f;
         if (need) m = m_new;
-        const float nm = ((m == -INFINITY) ? 0.f : -m) + kPackBiasLog2;
+        const float nm = ((m == -INFINITY) ? 0.f : -m) + (kScaled ? kPShift : kPackBiasLog2);
         // O holds sum_{i<j} P_i V_i of this piece once PV(j-1) completes;
         // rescale it when this block raised the max.  PV of the previous block
         // must also be done before P is overwritten below.
@@ -703,7 +713,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               // kScaled: two sums per half, else four
               const int k = kScaled ? 2 * c + (i & 1) : i;
               sum2[k] = f2_add(sum2[k], f2_pack(a, b));
-              pk[i] = pack_bf16x2_trunc(a, b);
+              pk[i] = kScaled ? pack_f16x2(a, b) : pack_bf16x2_trunc(a, b);
             }
             st_shared_v4(prow + uint32_t(c * SUB_BYTES) + (uint32_t(ch ^ (r & 7)) << 4), pk[0],
                          pk[1], pk[2], pk[3]);
@@ -715,8 +725,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if constexpr (kScaled)
           l = l * alpha +
-              (sum4(sum2[0], sum2[1]) * sc[0].inv_v + sum4(sum2[2], sum2[3]) * sc[1].inv_v) *
-                  kPackBiasInv;
+              (sum4(sum2[0], sum2[1]) * sc[0].inv_v + sum4(sum2[2], sum2[3]) * sc[1].inv_v);
         else
           l = l * alpha + sum8(sum2) * kPackBiasInv;
         tmem_wait_st();  // O rescale stores, if any
@@ -874,7 +883,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (q < p.q_len && p.lse)
         p.lse[size_t(h) * p.q_len + q] =
-            (l > 0.f) ? (m + __log2f(l)) * 0.69314718055994530942f : -INFINITY;
+            (l > 0.f) ? (m - (kScaled ? kPShift : 0.f) + __log2f(l)) * 0.69314718055994530942f
+                      : -INFINITY;
     }
     bulk_wait_group0();  // this thread's output stores (if any) have completed
     // query tiles without any visible block: all their rows are fully masked

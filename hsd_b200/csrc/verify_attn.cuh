@@ -7,7 +7,7 @@
 namespace hsd {
 namespace attn {
 
-// Scales of 64 columns of one KV head: scores times k; V scale v.
+// Scales of 64 columns of one KV head: scores times k; V (held in fp16) times v.
 struct __align__(16) ColumnScale {
   float score;   // k * softmax scale * log2 e
   float log2_v;  // log2 v
@@ -22,8 +22,8 @@ namespace hsd_host {
 
 // Checked arguments of hsd_verify_attention; partials, flags and sync are the
 // stream-K scratch (all null: one CTA per item); with
-// col_scale [num_kv_heads][2 ceil(kv_len / 128)], k and v hold values that the
-// scales multiply, and `scale` is not used.
+// col_scale [num_kv_heads][2 ceil(kv_len / 128)], k (bf16) and v (fp16) hold values
+// that the scales multiply, and `scale` is not used.
 struct AttentionArgs {
   const void *q, *k, *v;
   int64_t q_row_stride, q_head_stride, k_row_stride, k_head_stride, v_row_stride, v_head_stride;
