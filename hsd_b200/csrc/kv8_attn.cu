@@ -198,11 +198,18 @@ ManyLayout many_layout(int32_t kv_len, int32_t hkv) {
 // heads, 1600 columns: 128 rows 18 / 42, 256 rows 34 / 40, 384 rows 36 / 35; 8192
 // columns: 32 rows 32 / 63, 128 rows 58 / 62, 256 rows 112 / 53; 16/8 heads, 32768
 // columns: 32 rows 61 / 115, 128 rows 207 / 113.
-bool use_rows(int32_t q_len, int32_t kv_len, int32_t hq, int32_t hkv) {
+struct Path {
+  int splits;  // rows kernel: CTAs per tile; 0: many rows
+  size_t bytes;
+};
+Path choose_path(int32_t q_len, int32_t kv_len, int32_t hq, int32_t hkv) {
   const float tiles = float((q_len + 127) / 128) * float((hq / hkv + 1) / 2) * float(hkv);
   const float many = 40.f + 1.3e-4f * float(kv_len) * float(hkv) +
                      tiles * float((kv_len + 127) / 128) * (2.4f / 148.f);
-  return hsd_host::kv8_rows_us(q_len, kv_len, hq, hkv) <= many;
+  const hsd_host::Kv8RowsChoice rows = hsd_host::kv8_rows_choose(q_len, kv_len, hq, hkv);
+  if (rows.us <= many)
+    return {rows.splits, hsd_host::kv8_rows_workspace_bytes(q_len, hq, hkv, rows.splits)};
+  return {0, many_layout(kv_len, hkv).total};
 }
 
 int many_launch(const hsd_host::Kv8AttnArgs& a, const hsd_plan_t& plan, float scale) {
@@ -282,9 +289,7 @@ extern "C" size_t hsd_kv8_attention_workspace_bytes(int32_t q_len, int32_t kv_le
   if (q_len <= 0 || kv_len <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 ||
       num_q_heads % num_kv_heads)
     return 0;
-  if (use_rows(q_len, kv_len, num_q_heads, num_kv_heads))
-    return hsd_host::kv8_rows_workspace_bytes(q_len, kv_len, num_q_heads, num_kv_heads);
-  return many_layout(kv_len, num_kv_heads).total;
+  return choose_path(q_len, kv_len, num_q_heads, num_kv_heads).bytes;
 }
 
 extern "C" int hsd_verify_attention_kv8(
@@ -326,12 +331,12 @@ extern "C" int hsd_verify_attention_kv8(
         plan ? plan->kv_len : -1, sealed, tail_row0);
     return HSD_ERR_INVALID_ARG;
   }
-  const size_t need =
-      hsd_kv8_attention_workspace_bytes(q_len, kv_len, num_q_heads, num_kv_heads);
-  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) || workspace_bytes < need) {
+  const Path path = choose_path(q_len, kv_len, num_q_heads, num_kv_heads);
+  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) ||
+      workspace_bytes < path.bytes) {
     hsd_host::set_error(
         "hsd_verify_attention_kv8: workspace %zu bytes (need %zu, 256-byte aligned)",
-        workspace_bytes, need);
+        workspace_bytes, path.bytes);
     return HSD_ERR_INVALID_ARG;
   }
   hsd_host::Kv8AttnArgs a;
@@ -370,6 +375,5 @@ extern "C" int hsd_verify_attention_kv8(
   a.vt_head_stride = vt_head_stride;
   a.workspace = workspace;
   a.stream = reinterpret_cast<cudaStream_t>(stream);
-  return use_rows(q_len, kv_len, num_q_heads, num_kv_heads) ? hsd_host::kv8_rows_launch(a)
-                                                             : many_launch(a, *plan, scale);
+  return path.splits ? hsd_host::kv8_rows_launch(a, path.splits) : many_launch(a, *plan, scale);
 }

@@ -79,10 +79,14 @@ struct Kv8AttnArgs {
   void* workspace;
   cudaStream_t stream;
 };
-// What the rows kernel takes for these sizes, by its own model.
-float kv8_rows_us(int q_len, int kv_len, int hq, int hkv);
-size_t kv8_rows_workspace_bytes(int q_len, int kv_len, int hq, int hkv);
-int kv8_rows_launch(const Kv8AttnArgs& a);
+// CTAs per tile of the rows kernel for these sizes, and its time by its own model.
+struct Kv8RowsChoice {
+  int splits;
+  float us;
+};
+Kv8RowsChoice kv8_rows_choose(int q_len, int kv_len, int hq, int hkv);
+size_t kv8_rows_workspace_bytes(int q_len, int hq, int hkv, int splits);
+int kv8_rows_launch(const Kv8AttnArgs& a, int splits);
 // 3-D map {128 dims, rows, heads} of int8 (box 128 x box_rows) or bf16 (box
 // 64 x box_rows), 128-byte swizzle.
 int kv8_map(CUtensorMap* map, const void* base, bool bf16, int64_t rows, int heads,

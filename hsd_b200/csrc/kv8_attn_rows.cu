@@ -41,6 +41,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <mutex>
 
 namespace hsd {
 namespace kv8r {
@@ -814,34 +815,50 @@ int n_tiles(int q_len, int group) {
   const int r = tile_rows(q_len, group);
   return int((int64_t(q_len) * group + r - 1) / r);
 }
-std::atomic<int> g_clusters[2][kMaxDevices][kv8r::kMaxCluster + 1];
+// What the current device runs at once, looked up once per device.
+struct Device {
+  int sms = 148;
+  int clusters[2][kv8r::kMaxCluster + 1];  // [16 rows][CTAs of a cluster]
+};
 
-// Clusters of s CTAs that the current device runs at once (SMs of a cluster lie
-// in one group of the chip, so this is less than SMs / s).
-int resident_clusters(bool wide, int s) {
-  const int sms = kv8_sm_count();
+// Clusters of s CTAs at once: SMs of a cluster lie in one group of the chip, so
+// this is less than SMs / s.
+int resident_clusters(bool wide, int s, int dev, int sms) {
+  if (s == 1 || set_rows_attribute(wide, dev) != HSD_OK) return sms / s;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(s * sms));
+  cfg.blockDim = dim3(kv8r::kThreads);
+  cfg.dynamicSmemBytes = kv8r::kSmem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = unsigned(s);
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  return cudaOccupancyMaxActiveClusters(&n, rows_kernel_of(wide), &cfg) == cudaSuccess && n > 0
+             ? n
+             : sms / s;
+}
+
+const Device& current_device() {
+  static Device table[kMaxDevices + 1];  // the last: no device
+  static std::once_flag once[kMaxDevices + 1];
   int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return sms / s;
-  int n = g_clusters[wide][dev][s].load(std::memory_order_relaxed);
-  if (n > 0) return n;
-  n = sms / s;
-  if (s > 1 && set_rows_attribute(wide, dev) == HSD_OK) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(unsigned(s * sms));
-    cfg.blockDim = dim3(kv8r::kThreads);
-    cfg.dynamicSmemBytes = kv8r::kSmem;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = unsigned(s);
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    int m = 0;
-    if (cudaOccupancyMaxActiveClusters(&m, rows_kernel_of(wide), &cfg) == cudaSuccess && m > 0)
-      n = m;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) {
+    cudaGetLastError();
+    dev = kMaxDevices;
   }
-  if (cudaGetLastError() == cudaSuccess) g_clusters[wide][dev][s].store(n);
-  return n;
+  std::call_once(once[dev], [dev] {
+    Device& d = table[dev];
+    if (dev < kMaxDevices) d.sms = kv8_sm_count();
+    for (int wide = 0; wide < 2; ++wide)
+      for (int s = 1; s <= kv8r::kMaxCluster; ++s)
+        d.clusters[wide][s] =
+            dev < kMaxDevices ? resident_clusters(wide, s, dev, d.sms) : d.sms / s;
+    cudaGetLastError();
+  });
+  return table[dev];
 }
 
 // CTAs per tile and what the launch then takes.  With every SM busy a warp's step
@@ -849,11 +866,8 @@ int resident_clusters(bool wide, int s) {
 // to 32768 columns), so the time goes by the waves of clusters and the steps of a
 // warp; more than kMaxCluster CTAs per tile, when there are few tiles, need the
 // join kernel (4 us).
-struct Choice {
-  int splits;
-  float us;
-};
-Choice choose(int q_len, int kv_len, int hq, int hkv) {
+Kv8RowsChoice choose(int q_len, int kv_len, int hq, int hkv) {
+  const Device& dev = current_device();
   const int64_t tiles = int64_t(n_tiles(q_len, hq / hkv)) * hkv;
   const bool wide = tile_rows(q_len, hq / hkv) > 8;
   const int units = (kv_len + 63) / 64;
@@ -862,27 +876,27 @@ Choice choose(int q_len, int kv_len, int hq, int hkv) {
     const int steps = (units + s * kv8r::kWarps - 1) / (s * kv8r::kWarps);
     return float(waves) * (5.f + (wide ? 3.3f : 2.f) * float(steps));
   };
-  Choice best{1, time((tiles + kv8_sm_count() - 1) / kv8_sm_count(), 1)};
+  Kv8RowsChoice best{1, time((tiles + dev.sms - 1) / dev.sms, 1)};
   for (int s = 2; s <= kv8r::kMaxCluster && s <= most; ++s) {
-    const int at_once = resident_clusters(wide, s);
+    const int at_once = dev.clusters[wide][s];
     const float us = time((tiles + at_once - 1) / at_once, s);
     if (us < best.us) best = {s, us};
   }
-  const int64_t s = std::min<int64_t>(kv8_sm_count() / tiles, most);
+  const int64_t s = std::min<int64_t>(dev.sms / tiles, most);
   if (s > kv8r::kMaxCluster && time(1, int(s)) + 4.f < best.us)
     best = {int(s), time(1, int(s)) + 4.f};
   return best;
 }
 }  // namespace
 
-float kv8_rows_us(int q_len, int kv_len, int hq, int hkv) {
-  return choose(q_len, kv_len, hq, hkv).us;
+Kv8RowsChoice kv8_rows_choose(int q_len, int kv_len, int hq, int hkv) {
+  return choose(q_len, kv_len, hq, hkv);
 }
 
-size_t kv8_rows_workspace_bytes(int q_len, int kv_len, int hq, int hkv) {
-  const int s = choose(q_len, kv_len, hq, hkv).splits;
-  if (s <= kv8r::kMaxCluster) return kKv8FlagBytes;
-  return kKv8FlagBytes + size_t(n_tiles(q_len, hq / hkv)) * hkv * s * kv8r::kRecord * sizeof(float);
+size_t kv8_rows_workspace_bytes(int q_len, int hq, int hkv, int splits) {
+  if (splits <= kv8r::kMaxCluster) return kKv8FlagBytes;
+  return kKv8FlagBytes +
+         size_t(n_tiles(q_len, hq / hkv)) * hkv * splits * kv8r::kRecord * sizeof(float);
 }
 
 int kv8_map(CUtensorMap* map, const void* base, bool bf16, int64_t rows, int heads,
@@ -917,7 +931,7 @@ int kv8_sm_count() {
   return n;
 }
 
-int kv8_rows_launch(const Kv8AttnArgs& a) {
+int kv8_rows_launch(const Kv8AttnArgs& a, int splits) {
   const hsd::kv8a::Params& p = a.p;
   CUtensorMap k8, v8, kt, vt;
   const int64_t tail_rows = p.kv_len - p.tail_row0;
@@ -947,7 +961,7 @@ int kv8_rows_launch(const Kv8AttnArgs& a) {
   kv8r::Split sp;
   sp.n_tiles = n_tiles(p.q_len, p.group);
   sp.rows = tile_rows(p.q_len, p.group);
-  sp.splits = choose(p.q_len, p.kv_len, p.hq, p.hkv).splits;
+  sp.splits = splits;
   const bool cluster = sp.splits > 1 && sp.splits <= kv8r::kMaxCluster;
   sp.partials = sp.splits > kv8r::kMaxCluster
                     ? reinterpret_cast<float*>(static_cast<char*>(a.workspace) + kKv8FlagBytes)
