@@ -570,12 +570,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t mw[4] = {uint32_t(wd_next[0]), uint32_t(wd_next[0] >> 32), uint32_t(wd_next[1]),
                           uint32_t(wd_next[1] >> 32)};
         if (j + 1 < pc.b1) e_next = list[j + 1];
-        const ColumnScale* sc = sm.scales[nb & (NSCALE - 1)];
-        if constexpr (kScaled) ++nb;
         ok = __all_sync(0xffffffffu, mbar_wait(&sm.bar_s_full[s], uint32_t(gs) & 1u, abort,
                                                p.status, 0x300 + s));
         if (!ok) break;
         tc_fence_after();
+        ColumnScale sc[2];  // of the halves, in registers over the block
+        if constexpr (kScaled) {
+          sc[0] = sm.scales[nb & (NSCALE - 1)][0];
+          sc[1] = sm.scales[nb & (NSCALE - 1)][1];
+          ++nb;
+        }
         // S row -> registers: four loads in flight, one wait
         uint32_t u[4][32];
 #pragma unroll
