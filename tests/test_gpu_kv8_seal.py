@@ -125,3 +125,24 @@ def test_replayed_graph_seals_what_the_planes_hold_then(dev):
         graph.replay()
         torch.cuda.synchronize()
         _check(kv8, x, 0, 64)
+
+
+def test_offsets_past_32_bits(dev):
+    """The last plane of a cache of more than 2^31 bytes."""
+    from hsd_b200.compaction import plane_pointers
+    from hsd_b200.kv8 import Kv8Cache
+    cap = 9 * 2 ** 20                     # 9 M rows x 128 = 1.2e9 bytes a plane
+    kv8 = Kv8Cache(1, 1, cap, device=dev)
+    g = torch.Generator().manual_seed(5)
+    x = torch.randn(2, 1, 128, 128, generator=g).to(torch.bfloat16).to(dev)
+    kv8.sealed = cap - 128
+    kv8.seal(plane_pointers([x[0], x[1]]), 128, src_row0=0)
+    n, s = OK.seal(x.cpu())
+    assert np.array_equal(kv8.data[0, :, :, -128:].cpu().numpy(), n)
+    assert np.array_equal(kv8.scale[0, :, :, -2:].cpu().numpy(), s.astype(np.float32))
+    assert not kv8.data[0, :, :, -192:-128].any()
+    back = torch.zeros_like(x)
+    kv8.unseal(plane_pointers([back[0], back[1]]), cap - 100, 100, dst_row0=28)
+    want = (torch.from_numpy(n).float() * torch.from_numpy(s.astype(np.float32)).repeat_interleave(
+        64, -1)[..., None]).to(torch.bfloat16).to(dev)
+    assert torch.equal(back[:, :, 28:], want[:, :, 28:]) and not back[:, :, :28].any()

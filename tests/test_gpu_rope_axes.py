@@ -156,3 +156,49 @@ def test_bad_pair_axis_is_reported(dev):
                      kc.clone(), 0, status=st)
     assert int(st.item()) & N.HSD_DEV_BAD_INDEX
     assert torch.equal(y[:, [5, 69]], x[:, [5, 69]]) and not torch.equal(y[:, 4], x[:, 4])
+
+
+def test_cache_offsets_past_32_bits(dev):
+    """The last head's rows of caches of more than 2^31 elements."""
+    from hsd_b200.rope import RotaryAxes, rope_append_axes
+    rot = RotaryAxes([64], device=dev)
+    kc = torch.empty(2, 9 * 2 ** 20, 128, dtype=torch.bfloat16, device=dev)
+    vc = torch.empty_like(kc)
+    n = 5
+    row0 = kc.shape[1] - n
+    x = torch.randn(n, 256, device=dev).to(torch.bfloat16)
+    rope_append_axes(None, x, x, torch.zeros(1, n, dtype=torch.int64, device=dev), rot, kc, vc,
+                     row0)
+    for c in (kc, vc):
+        assert torch.equal(c[:, row0:].transpose(0, 1).reshape(n, 256), x)
+
+
+def test_refusals(dev):
+    """Every refusal of the binding, on real tensors; nothing is launched."""
+    from hsd_b200 import _native as N
+    from hsd_b200.rope import RotaryAxes, rope_append_axes
+    rot = RotaryAxes([32, 32], device=dev)
+    x = torch.zeros(4, 256, dtype=torch.bfloat16, device=dev)
+    kc = torch.zeros(2, 8, 128, dtype=torch.bfloat16, device=dev)
+    pos = torch.zeros(2, 4, dtype=torch.int64, device=dev)
+    ok = dict(q=x, k=x.clone(), v=x.clone(), positions=pos, rotary=rot, k_cache=kc,
+              v_cache=kc.clone(), dst_row0=4)
+    bad = [
+        dict(q=x.float()), dict(q=x[:3]), dict(q=x[:, :200]), dict(q=x.cpu()), dict(k=x[:3]),
+        dict(k=x[:, :128]), dict(v=x[:3]), dict(k=x.t().contiguous().t()), dict(positions=pos[:1]),
+        dict(positions=pos[:, :3]), dict(positions=pos.float()), dict(positions=pos.cpu()),
+        dict(positions=pos[None, None]), dict(dst_row0=5), dict(dst_row0=-1),
+        dict(k_cache=kc[:1]), dict(k_cache=kc.float()), dict(k_cache=kc.cpu()),
+        dict(k_cache=kc[:, :, :64]), dict(v_cache=torch.zeros(2, 9, 128, dtype=torch.bfloat16,
+                                                             device=dev)),
+        dict(q=None, out=x), dict(out=x[:3]), dict(out=x.float()), dict(num_q_heads=3),
+        dict(num_kv_heads=1), dict(rotary=RotaryAxes([32, 32], device="cpu")),
+        dict(status=torch.zeros(1, device=dev)),
+        dict(out=torch.zeros(256, 4, dtype=torch.bfloat16, device=dev).t()),
+    ]
+    for change in bad:
+        with pytest.raises((ValueError, TypeError, N.HSDError)):
+            rope_append_axes(**{**ok, **change})
+    assert not kc.any()
+    rope_append_axes(**ok)
+    torch.cuda.synchronize()
