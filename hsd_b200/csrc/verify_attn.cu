@@ -278,8 +278,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int per_tile = p.hkv * p.pairs;
 
   if (threadIdx.x == 0) {
-    // Q and every K/V stage are released by both MMA issuers (one per slot;
-    // the slot-0 issuer releases twice when slot 1 has no head in a piece)
+    // Q and every K/V stage are released by both MMA issuers (one per slot)
     mbar_init(&sm.bar_q, 1);
     mbar_init(&sm.bar_q_free, NSLOT);
     for (int i = 0; i < NSTAGE; ++i) {
@@ -421,16 +420,25 @@ __global__ void __launch_bounds__(kThreads, 1)
       Piece pc;
       while (ok && next_piece(p, w, w1, pc)) {
         const int n_loads = 2 * (pc.b1 - pc.b0);
-        if (s >= pc.nslot) {  // no head of this piece in slot 1: skip its FIFO entries
-          for (int i = 0; i < n_loads; ++i)
+        if (s >= pc.nslot) {
+          // No head of this piece in slot 1: its tiles are waited for and released
+          // all the same.  Skipping them would let this thread wait for a phase
+          // two ahead of the barrier's, which the parity cannot tell from the last.
+          ok = mbar_wait(&sm.bar_q, uint32_t(pieces) & 1u, abort, p.status, 0x20c);
+          if (!ok) break;
+          mbar_arrive(&sm.bar_q_free);
+          for (int i = 0; i < n_loads && ok; ++i) {
+            ok = mbar_wait(&sm.bar_full[stage], phase, abort, p.status, 0x20e);
+            if (!ok) break;
+            mbar_arrive(&sm.bar_empty[stage]);
             if (++stage == NSTAGE) {
               stage = 0;
               phase ^= 1u;
             }
+          }
           ++pieces;
           continue;
         }
-        const int rel = pc.nslot == NSLOT ? 1 : NSLOT;  // releases owed per stage
         ok = mbar_wait(&sm.bar_q, uint32_t(pieces) & 1u, abort, p.status, 0x200 + s);
         if (!ok) break;
         tc_fence_after();
@@ -459,8 +467,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             ++ns;
             // the piece's last S: Q is free once it completes, so the next
             // piece's Q loads under this block's softmax and PV
-            if (j == pc.b1 - 1)
-              for (int k = 0; k < rel; ++k) umma_commit(&sm.bar_q_free);
+            if (j == pc.b1 - 1) umma_commit(&sm.bar_q_free);
           } else {
             ok = mbar_wait(&sm.bar_p_full[s], uint32_t(gs) & 1u, abort, p.status, 0x206 + s);
             if (!ok) break;
@@ -476,7 +483,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             ++gs;
           }
           issued_any = true;
-          for (int k = 0; k < rel; ++k) umma_commit(&sm.bar_empty[st]);
+          umma_commit(&sm.bar_empty[st]);
         }
         if (!ok) break;
         ++ps;
