@@ -128,7 +128,9 @@ __device__ __forceinline__ float byte_f(uint32_t w) {
   return float(int32_t(w << (24 - 8 * k)) >> 24);
 }
 
-// CTA (64-row group, plane); thread: 16 values at a time
+// CTA (64-row group, plane); thread: 8 values at a time, four in flight, so that
+// a warp's loads and stores are contiguous (16 values a thread, in two stores 32
+// bytes apart, took 23 us instead of 12 us for 112 planes x 2560 rows)
 __global__ void __launch_bounds__(kThreads)
     unseal_kernel(const int8_t* data, int64_t plane_stride, const float* scale,
                   int64_t scale_stride, int64_t row0, int n_rows, const uint64_t* dst_planes,
@@ -137,26 +139,32 @@ __global__ void __launch_bounds__(kThreads)
   const int64_t plane = blockIdx.y;
   const int64_t first = int64_t(blockIdx.x) * kBlockRows;  // row of the range
   const int rows = int(min(int64_t(kBlockRows), int64_t(n_rows) - first));
-  const int4* src = reinterpret_cast<const int4*>(data + plane * plane_stride +
-                                                  (row0 + first) * kDim);
+  const uint2* src =
+      reinterpret_cast<const uint2*>(data + plane * plane_stride + (row0 + first) * kDim);
   uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<char*>(dst_planes[plane]) +
                                         (dst_row0 + first) * (kDim * 2));
+  const float* sc = scale + plane * scale_stride;
+  constexpr int kUnits = kBlockRows * kDim / 8 / kThreads;
+  uint2 v[kUnits];
+  float s[kUnits];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int u = int(threadIdx.x) + kThreads * j;  // 8 units of 16 values per row
-    const int r = u >> 3;
-    if (r >= rows) continue;
-    const int4 v = __ldcs(src + u);
-    const float s = scale[plane * scale_stride + (row0 + first + r) / kBlockRows];
-    const uint32_t in[4] = {uint32_t(v.x), uint32_t(v.y), uint32_t(v.z), uint32_t(v.w)};
-    uint32_t o[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      o[2 * i] = pack_bf16x2(byte_f<0>(in[i]) * s, byte_f<1>(in[i]) * s);
-      o[2 * i + 1] = pack_bf16x2(byte_f<2>(in[i]) * s, byte_f<3>(in[i]) * s);
+  for (int j = 0; j < kUnits; ++j) {
+    const int u = int(threadIdx.x) + kThreads * j;  // 16 units of 8 values per row
+    const int r = u >> 4;
+    if (r < rows) {
+      v[j] = __ldcs(src + u);
+      s[j] = __ldg(sc + (row0 + first + r) / kBlockRows);
     }
-    dst[2 * u] = make_uint4(o[0], o[1], o[2], o[3]);
-    dst[2 * u + 1] = make_uint4(o[4], o[5], o[6], o[7]);
+  }
+#pragma unroll
+  for (int j = 0; j < kUnits; ++j) {
+    const int u = int(threadIdx.x) + kThreads * j;
+    // streamed: the rows are read once, later, and by another kernel
+    if ((u >> 4) < rows)
+      __stcs(dst + u, make_uint4(pack_bf16x2(byte_f<0>(v[j].x) * s[j], byte_f<1>(v[j].x) * s[j]),
+                                 pack_bf16x2(byte_f<2>(v[j].x) * s[j], byte_f<3>(v[j].x) * s[j]),
+                                 pack_bf16x2(byte_f<0>(v[j].y) * s[j], byte_f<1>(v[j].y) * s[j]),
+                                 pack_bf16x2(byte_f<2>(v[j].y) * s[j], byte_f<3>(v[j].y) * s[j])));
   }
 }
 

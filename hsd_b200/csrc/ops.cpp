@@ -10,6 +10,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -458,7 +459,7 @@ PyObject* verify_attention_kv8(PyObject* const* args, Py_ssize_t n_args) {
   const c10::cuda::CUDAGuard guard(dev);
   at::Tensor out, lse;
   if (a.none(9)) {
-    out = at::empty({q_len, hq, 128}, q.keep.options());
+    out = at::detail::empty_cuda({q_len, hq, 128}, at::kBFloat16, dev, std::nullopt);
   } else {
     out = a.tensor(9, "out");
     if (out.scalar_type() != at::kBFloat16 || out.dim() != 3 || out.size(0) != q_len ||
@@ -468,7 +469,7 @@ PyObject* verify_attention_kv8(PyObject* const* args, Py_ssize_t n_args) {
   }
   if (need_lse) {
     if (a.none(10)) {
-      lse = at::empty({hq, q_len}, q.keep.options().dtype(at::kFloat));
+      lse = at::detail::empty_cuda({hq, q_len}, at::kFloat, dev, std::nullopt);
     } else {
       lse = a.tensor(10, "lse");
       if (lse.scalar_type() != at::kFloat || lse.dim() != 2 || lse.size(0) != hq ||
