@@ -37,16 +37,30 @@ struct ExpandParams {
 constexpr int kExpandThreads = 256;
 constexpr float kMinVScale = 8.077935669463161e-28f;  // 2^-90
 
-// Columns of a 64-column tile that some query row sees.
+// Columns of a 64-column tile that some query row sees: a warp per query tile, four
+// tiles' loads in flight.
 __device__ __forceinline__ uint64_t seen_columns(const ExpandParams& p, int t, uint32_t* red) {
   if (threadIdx.x < 2) red[threadIdx.x] = 0u;
   __syncthreads();
+  constexpr int kWarps = kExpandThreads / 32;
   uint64_t w = 0ull;
-  for (int i = threadIdx.x; i < p.n_qtiles * 128; i += kExpandThreads) {
-    const size_t tile = size_t(i >> 7) * p.n_kv64 + t;
-    const int cls = p.tile_class[tile];
-    if (cls == 2) w = ~0ull;
-    if (cls == 1) w |= p.mask_words[tile * 128 + (i & 127)];
+  for (int q0 = warp_id(); q0 < p.n_qtiles; q0 += 4 * kWarps) {
+    int cls[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int qt = q0 + u * kWarps;
+      cls[u] = qt < p.n_qtiles ? p.tile_class[size_t(qt) * p.n_kv64 + t] : 0;
+    }
+    uint64_t m[4][4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        m[u][i] = cls[u] == 1 ? p.mask_words[(size_t(q0 + u * kWarps) * p.n_kv64 + t) * 128 +
+                                             32 * i + lane_id()]
+                              : (cls[u] == 2 ? ~0ull : 0ull);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) w |= (m[u][0] | m[u][1]) | (m[u][2] | m[u][3]);
   }
   const uint32_t lo = __reduce_or_sync(0xffffffffu, uint32_t(w));
   const uint32_t hi = __reduce_or_sync(0xffffffffu, uint32_t(w >> 32));
@@ -106,8 +120,6 @@ __global__ void __launch_bounds__(kExpandThreads) expand_kernel(const ExpandPara
       dst[at + 1] = make_uint4(o[4], o[5], o[6], o[7]);
     }
   } else {
-    // what stands in columns that no row sees must not reach the sums (0 * V)
-    const uint64_t seen = z == 1 ? seen_columns(p, t, red) : ~0ull;
     const __nv_bfloat16* src = p.tail[z] + h * p.head_stride[z] +
                                int64_t(col0 - p.tail_row0) * p.row_stride[z] + (tid & 15) * 8;
     const int rows = min(64, p.kv_len - col0);
@@ -116,8 +128,14 @@ __global__ void __launch_bounds__(kExpandThreads) expand_kernel(const ExpandPara
     for (int u = 0; u < 4; ++u) {
       const int r = 16 * u + (tid >> 4);
       v[u] = make_uint4(0u, 0u, 0u, 0u);
-      if (r < rows && ((seen >> r) & 1ull))
-        v[u] = __ldg(reinterpret_cast<const uint4*>(src + r * p.row_stride[z]));
+      if (r < rows) v[u] = __ldg(reinterpret_cast<const uint4*>(src + r * p.row_stride[z]));
+    }
+    if (z == 1) {
+      // what stands in columns that no row sees must not reach the sums (0 * V)
+      const uint64_t seen = seen_columns(p, t, red);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (!((seen >> (16 * u + (tid >> 4))) & 1ull)) v[u] = make_uint4(0u, 0u, 0u, 0u);
     }
     if (z == 1) {
       // the block's largest finite magnitude, as bf16 bits
