@@ -211,9 +211,11 @@ __device__ __forceinline__ bool next_piece(const Params& p, int& w, int w1, Piec
   return true;
 }
 
-// First work index of CTA k in stream-K mode.
+// First work index of CTA k in stream-K mode: floor(k total / g) without the 64-bit
+// product (g is the SM count, so k (total mod g) stays within 32 bits).
 __device__ __forceinline__ int range_start(int k, int total, int g) {
-  return int((int64_t(k) * total) / g);
+  const int each = total / g;
+  return k * each + int(uint32_t(k) * uint32_t(total - each * g) / uint32_t(g));
 }
 
 constexpr uint32_t kIdescS = idesc_bf16_f32(BM, BN, false, false);  // Q K^T: both K-major
@@ -344,6 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tma_prefetch_desc(&tm_q);
       tma_prefetch_desc(&tm_k);
       tma_prefetch_desc(&tm_v);
+      tma_prefetch_desc(&tm_o);
       int stage = 0;
       uint32_t phase = 0;
       int issued = 0;  // K/V tiles issued; ring slot i was used ceil((issued - i) / NSTAGE) times
@@ -783,9 +786,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t stg = smem_u32(sm.pb[s]) + uint32_t(r) * 16u;
         if constexpr (kScaled) {
           // fp16 times the power of two at or below the row's largest |O / l|
-          float top = 0.f;
+          float t4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int i = 0; i < 128; ++i) top = fmaxf(top, fabsf(o[i]));
+          for (int i = 0; i < 128; i += 8)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              t4[k] = fmax3(t4[k], fabsf(o[i + k]), fabsf(o[i + 4 + k]));
+          const float top = fmaxf(fmax3(t4[0], t4[1], t4[2]), t4[3]);
           const uint32_t unit =
               min(max(__float_as_uint(top * invl) & 0x7f800000u, 27u << 23), 247u << 23);
           const float f = invl * __uint_as_float((254u << 23) - unit);
@@ -888,12 +895,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             tma_store_3d(&tm_o, sm.pb[s], 0, qt * BM, h);
             tma_store_3d(&tm_o, sm.pb[s] + SUB_BYTES, 64, qt * BM, h);
             bulk_commit_group();
-            bulk_wait_group_read0();
+            if (w < w1) bulk_wait_group_read0();
           }
           mbar_arrive(&sm.bar_ofree[s]);  // also after an abort, so no thread waits long
         }
-        ok = __all_sync(0xffffffffu, mbar_wait(&sm.bar_ofree[s], uint32_t(fo) & 1u, abort,
-                                               p.status, 0x342 + s));
+        if (w < w1)  // after the last piece nothing overwrites the buffer
+          ok = __all_sync(0xffffffffu, mbar_wait(&sm.bar_ofree[s], uint32_t(fo) & 1u, abort,
+                                                 p.status, 0x342 + s));
         ++fo;
         if (!ok) break;
       }
