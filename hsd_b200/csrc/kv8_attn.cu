@@ -9,10 +9,16 @@
 // becomes bf16 (int8: the same integers, exactly; the bf16 tail copied), V fp16
 // (int8 exactly; 64 tail rows times the power of two that brings their largest
 // value to [64, 128): exact down to 2^-21 of it, else within 2^-31 of it), so that
-// P can be fp16 and keep 11 bits.  The expansion is bound by HBM and L2: 1 byte
-// read and 2 written per sealed value, and the attention finds it in L2.
+// P can be fp16 and keep 11 bits.  The expansion reads 1 byte and writes 2 per
+// sealed value, and the attention finds it in L2; for a region step's 4800 columns of
+// 2 heads it is latency (7.1 us alone from cold caches, about 3.5 in a stream of steps,
+// where the attention's setup runs under it).  Both together: 53.2 us for 2176 rows,
+// 12/2 heads, 4800 columns (the bf16 kernel alone 47.8), 217 us for 2049 rows and
+// 18,450 columns (210).
 #include "kv8_attn.cuh"
 #include "verify_attn.cuh"
+
+#include <algorithm>
 
 #include <cuda_fp16.h>
 
@@ -209,22 +215,25 @@ ManyLayout many_layout(int32_t kv_len, int32_t hkv) {
   return m;
 }
 
-// Rows kernel or many rows, by the time each takes.  Many rows: 40 us however
-// small (items cut between all SMs and joined by their first CTA one after
-// another), the expansion (1.3e-4 us a column and KV head), and 2.4 us per SM for
-// every 128 rows x 128 columns x two heads.  Measured (rows / many, us): 12/2
-// heads, 1600 columns: 128 rows 18 / 42, 256 rows 34 / 40, 384 rows 36 / 35; 8192
-// columns: 32 rows 32 / 63, 128 rows 58 / 62, 256 rows 112 / 53; 16/8 heads, 32768
-// columns: 32 rows 61 / 115, 128 rows 207 / 113.
+// Rows kernel or many rows, by the time each takes.  Many rows: 24 us, the expansion
+// (1.3e-4 us a column and KV head), 2.05 us per SM for every 128 rows x 128 columns x
+// two heads, and 1.2 us for each part of an item (128 rows, two heads) that its first
+// CTA merges when all SMs share few items.  Measured (rows / many, us): 12/2 heads, 1600
+// columns: 128 rows 18 / 38, 256 rows 37 / 38, 384 rows 36 / 32; 8192 columns: 64 rows
+// 36 / 60, 128 rows 58 / 60, 256 rows 101 / 50; 16/8 heads, 32768 columns: 32 rows 62 /
+// 113, 128 rows 207 / 113; 8/1 heads, 32768 columns: 64 rows 62 / 88, 128 rows 111 / 88.
 struct Path {
   int splits;  // rows kernel: CTAs per tile; 0: many rows
   size_t bytes;
 };
 Path choose_path(int32_t q_len, int32_t kv_len, int32_t hq, int32_t hkv) {
-  const float tiles = float((q_len + 127) / 128) * float((hq / hkv + 1) / 2) * float(hkv);
-  const float many = 40.f + 1.3e-4f * float(kv_len) * float(hkv) +
-                     tiles * float((kv_len + 127) / 128) * (2.4f / 148.f);
   const hsd_host::Kv8RowsChoice rows = hsd_host::kv8_rows_choose(q_len, kv_len, hq, hkv);
+  const float sms = float(rows.sms);
+  const float items = float((q_len + 127) / 128) * float((hq / hkv + 1) / 2) * float(hkv);
+  const float blocks = float((kv_len + 127) / 128);
+  const float merges = std::max(std::min(blocks, sms / items) - 1.f, 0.f);
+  const float many = 24.f + 1.3e-4f * float(kv_len) * float(hkv) +
+                     2.05f * items * blocks / sms + 1.2f * merges;
   if (rows.us <= many)
     return {rows.splits, hsd_host::kv8_rows_workspace_bytes(q_len, hq, hkv, rows.splits)};
   return {0, many_layout(kv_len, hkv).total};

@@ -79,10 +79,12 @@ struct Kv8AttnArgs {
   void* workspace;
   cudaStream_t stream;
 };
-// CTAs per tile of the rows kernel for these sizes, and its time by its own model.
+// CTAs per tile of the rows kernel for these sizes, its time by its own model, and
+// the device's SMs.
 struct Kv8RowsChoice {
   int splits;
   float us;
+  int sms;
 };
 Kv8RowsChoice kv8_rows_choose(int q_len, int kv_len, int hq, int hkv);
 size_t kv8_rows_workspace_bytes(int q_len, int hq, int hkv, int splits);
@@ -91,5 +93,4 @@ int kv8_rows_launch(const Kv8AttnArgs& a, int splits);
 // 64 x box_rows), 128-byte swizzle.
 int kv8_map(CUtensorMap* map, const void* base, bool bf16, int64_t rows, int heads,
             int64_t row_stride, int64_t head_stride, int box_rows, const char* what);
-int kv8_sm_count();
 }  // namespace hsd_host

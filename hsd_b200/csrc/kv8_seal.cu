@@ -16,7 +16,9 @@
 //
 // Seal: HBM bound, 2 bytes read and 1 written per value.  One CTA per block:
 // the block's 16 KB sit in registers between the maximum and the rounding, so
-// the rows are read once.  Unseal: 1 byte read, 2 written.
+// the rows are read once.  Unseal: 1 byte read, 2 written.  Measured: 28 layers of
+// 2 heads, 2560 rows (110 MB, partly in L2): seal 15.3 us, 7.2 TB/s; unseal 14.6 us,
+// 7.6 TB/s; 8 heads, 2048 rows (352 MB): 52.7 us, 6.7 TB/s and 53.9 us, 6.5 TB/s.
 #include "common.cuh"
 
 namespace hsd {
@@ -130,7 +132,7 @@ __device__ __forceinline__ float byte_f(uint32_t w) {
 
 // CTA (64-row group, plane); thread: 8 values at a time, four in flight, so that
 // a warp's loads and stores are contiguous (16 values a thread, in two stores 32
-// bytes apart, took 23 us instead of 12 us for 112 planes x 2560 rows)
+// bytes apart, took 23 us instead of 14 us for 112 planes x 2560 rows)
 __global__ void __launch_bounds__(kThreads)
     unseal_kernel(const int8_t* data, int64_t plane_stride, const float* scale,
                   int64_t scale_stride, int64_t row0, int n_rows, const uint64_t* dst_planes,

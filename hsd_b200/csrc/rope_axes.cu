@@ -19,7 +19,9 @@
 // Work: a CTA takes a few rows; 64 threads per row compute the row's cosines
 // and sines once into shared memory, and all heads use them.  The rows' first
 // loads are issued before, so they run under the trigonometry.  HBM bound:
-// each query, key and value row is read once and written once.
+// each query, key and value row is read once and written once.  Measured: 45.3 us
+// for 16640 rows of 16/8 heads (273 MB, 6.0 TB/s, 0.93 of a copy), 4.4 us for 2176
+// rows of 12/2 heads, 1.9 us (a launch) for one row.
 #include "common.cuh"
 
 namespace hsd {

@@ -111,9 +111,11 @@ def verify_attention_kv8(q, layer, sealed, k, v, plan: TilePlan, scale=None, tai
     Returns ``(out [Q, Hq, 128] bf16, lse [Hq, Q] fp32 natural log or None)``;
     rows that see nothing give 0 and -inf.
 
-    Runs on the device's current stream.  P is rounded to bf16 (as in
-    :func:`verify_attention`); scores, sums and the joined partial rows are
-    fp32.
+    Runs on the device's current stream, with scratch kept per device and
+    stream; with many rows it holds the layer's expanded columns (512 bytes
+    per column and KV head).  Scales must be positive, as sealing leaves them.
+    P is rounded to fp16 (few rows: to bf16 over the bf16 columns); scores and
+    sums are fp32.
     """
     return N.ops().verify_attention_kv8(q, layer, sealed, k, v, plan.address, plan.status, scale,
                                         tail_row0, out, lse, need_lse)

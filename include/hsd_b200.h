@@ -395,7 +395,12 @@ int hsd_kv8_unseal(const int8_t *data, int64_t plane_stride, const float *scale,
  * be empty, its pointers then NULL.  The mask, out, lse and the strides of q
  * and the tails are those of hsd_verify_attention; fully masked rows give 0
  * and -inf, and what stands in a bf16 column that no query row sees does not
- * matter.  P is rounded to bf16, everything else is fp32.
+ * matter.  Scales must be positive.  P is rounded to fp16 (few rows: to bf16
+ * over the bf16 columns); scores, sums and joined rows are fp32, the partial
+ * rows of items cut between SMs fp16 times a power of two per row.
+ * Two paths by size: few rows read the cache as it is; many first expand the
+ * layer's columns into the workspace, which then holds 512 bytes per column
+ * and KV head.
  * workspace: hsd_kv8_attention_workspace_bytes, 256-byte aligned, its first
  * 64 KB zero-filled before the first use; each call leaves it ready for the
  * next (after an error status, zero them again), and calls sharing one must

@@ -65,7 +65,8 @@ def test_both_sides_of_the_choice_agree(dev, q_len):
 
 
 @pytest.mark.parametrize("hq,density,seed", [(6, 0.5, 0), (6, 0.01, 1), (12, 0.3, 3),
-                                             (12, 0.005, 4), (12, 0.0, 2)])
+                                             (12, 0.005, 4), (12, 0.0, 2), (2, 0.5, 5),
+                                             (2, 0.01, 6)])
 def test_random_masks_and_empty_rows(dev, hq, density, seed):
     q_len, kv_len, sealed, hkv = 800, 1300, 640, 2
     g = torch.Generator().manual_seed(seed)
@@ -74,7 +75,7 @@ def test_random_masks_and_empty_rows(dev, hq, density, seed):
     allowed[128:256] = False              # a query tile that sees nothing
     allowed[:, 64:300] = False            # column tiles that nobody sees
     allowed = allowed.to(dev)
-    assert many(q_len, kv_len, hq, hkv) == (hq == 12)
+    assert many(q_len, kv_len, hq, hkv) == (hq > 2)
     x = T.make(dev, hq, hkv, q_len, kv_len, sealed, seed=seed)
     T.check(T.run(*x, sealed, T.plan_of(allowed)), T.exact(*x, sealed, allowed))
 
