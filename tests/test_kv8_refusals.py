@@ -56,6 +56,48 @@ def test_kv8_seal_c_checks():
         assert unseal(**bad) == 1, bad
 
 
+def test_verify_attention_kv8_c_checks():
+    lib = N.load()
+    plan = N.Plan()
+    plan.q_len, plan.kv_len = 64, 300
+
+    def call(q=A, q_row=1536, q_head=128, k8=A, h8=256 * 128, ks=A, sh=4, sealed=256, kt=A,
+             kt_row=128, kt_head=300 * 128, row0=0, out=A, lse=A, q_len=64, kv_len=300, hq=12, hkv=2,
+             d=128, scale=0.1, pl=C.byref(plan), ws=A, ws_bytes=0):
+        # ws_bytes = 0: what passes every other check is refused for its workspace
+        return lib.hsd_verify_attention_kv8(q, q_row, q_head, k8, h8, k8, h8, ks, ks, sh, sealed, kt,
+                                            kt_row, kt_head, kt, kt_row, kt_head, row0, out, lse,
+                                            q_len, kv_len, hq, hkv, d, scale, pl, ws, ws_bytes, None,
+                                            None)
+
+    def refused(word, code=1, **kw):
+        assert call(**kw) == code, kw
+        assert word in lib.hsd_last_error(), (kw, lib.hsd_last_error())
+
+    need = lib.hsd_kv8_attention_workspace_bytes(64, 300, 12, 2)
+    assert need >= 65536
+    refused(b"workspace")
+    refused(b"workspace", ws=None, ws_bytes=need)
+    refused(b"workspace", ws=C.c_void_p(128), ws_bytes=need)
+    refused(b"workspace", ws_bytes=need - 1)
+    refused(b"workspace", lse=None)
+    refused(b"workspace", row0=256, kt_head=44 * 128)
+    refused(b"workspace", sealed=0, k8=None, ks=None, h8=0, sh=0)
+    refused(b"head_dim", code=2, d=64)
+    for scale in (0.0, -0.1, math.nan, math.inf):
+        refused(b"scale", scale=scale)
+    for bad in (dict(pl=None), dict(q_len=65), dict(kv_len=299), dict(hq=0), dict(hkv=0), dict(hq=13),
+                dict(q=None), dict(q=C.c_void_p(8)), dict(q_row=1540), dict(q_head=0), dict(out=None),
+                dict(out=C.c_void_p(264)), dict(lse=C.c_void_p(258)), dict(sealed=-64),
+                dict(sealed=100), dict(sealed=320), dict(row0=-1), dict(row0=257), dict(k8=None),
+                dict(k8=C.c_void_p(264)), dict(ks=None), dict(ks=C.c_void_p(258)),
+                dict(h8=256 * 128 - 16), dict(h8=256 * 128 + 8), dict(sh=3), dict(kt=None),
+                dict(kt_row=132), dict(kt_head=0)):
+        refused(b"bad arguments", **bad)
+    for bad in ((0, 300, 12, 2), (64, 0, 12, 2), (64, 300, 0, 2), (64, 300, 12, 0), (64, 300, 12, 5)):
+        assert lib.hsd_kv8_attention_workspace_bytes(*bad) == 0
+
+
 def test_rotary_axes_refusals_and_tables():
     from hsd_b200.rope import RotaryAxes
     for bad in (dict(sections=[]), dict(sections=[32, 31]), dict(sections=[-1, 65]),
