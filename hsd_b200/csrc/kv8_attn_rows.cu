@@ -35,12 +35,14 @@
 //
 // Measured: one row, 16/8 heads, 131,051 columns (269 MB): 47 us and 4 us for the
 // join, 5.1 TB/s over both (0.79 of a copy; a wait of 3 to 4 us for the first tiles
-// and the join are what is left).  12/2 heads, 2625 columns: one row 8.5 us, forty
-// 13.4 us: latency (launch, block list, tile, join), not bytes.
+// and the join are what is left).  12/2 heads, 2625 columns: one row 7.7 us, forty
+// 13.2 us: latency (launch, block list, tile, join), not bytes.
 //
 // Join: warps of a CTA through shared memory; up to eight CTAs of a tile as a
-// cluster, each reading the others' rows from their shared memory; more through
-// fp32 partial rows in the workspace and a second small launch.  No counters
+// cluster, each writing its rows into the shared memory of the CTA that joins them
+// (reading them from there instead took a second barrier: one row 8.5 us for
+// 7.7); more through fp32 partial rows in the workspace and a second small
+// launch.  No counters
 // and no flags: the result does not depend on the order in which CTAs finish.
 #include "kv8_attn.cuh"
 
@@ -65,6 +67,7 @@ static_assert(kBuf == 3, "a step's K and V and the next step's K are issued befo
 constexpr int kRing = kBuf * kTile;  // a warp's buffers: K, V, K, V, ... in turn
 constexpr int kMaxRows = 16;
 constexpr int kMaxCluster = 8;
+constexpr int kMaxIn = 21;  // the most of s ceil(kMaxRows / s) for s <= kMaxCluster
 constexpr int kRecord = kMaxRows * HD + 2 * kMaxRows;  // floats of a partial record
 constexpr float kPShift = 15.0f;                 // P = 2^15 exp(s - max)
 
@@ -74,7 +77,9 @@ struct __align__(1024) Smem {
   uint2 qbf[8][2][32];
   float unit[kMaxRows];  // power of two of the row
   float2 ml[kWarps][kMaxRows];
-  float2 cta_ml[kMaxRows];  // the CTA's joined rows, for the other CTAs of the cluster
+  // rows that the cluster's CTAs hand to this one: [CTA][row / CTAs]
+  float4 in_rows[kMaxIn][HD / 4];
+  float2 in_ml[kMaxIn];
   uint64_t full[kWarps][kBuf];
   int abort;
 };
@@ -462,24 +467,19 @@ __device__ __forceinline__ uint32_t cluster_addr(const void* p, uint32_t rank) {
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
   return r;
 }
-__device__ __forceinline__ float4 ld_cluster_v4(uint32_t a) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(a)
+__device__ __forceinline__ void st_cluster_v4(uint32_t a, float4 v) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(a), "f"(v.x), "f"(v.y),
+               "f"(v.z), "f"(v.w)
                : "memory");
-  return v;
 }
-__device__ __forceinline__ float2 ld_cluster_v2(uint32_t a) {
-  float2 v;
-  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
-               : "=f"(v.x), "=f"(v.y)
-               : "r"(a)
-               : "memory");
-  return v;
+__device__ __forceinline__ void st_cluster_v2(uint32_t a, float x, float y) {
+  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(a), "f"(x), "f"(y) : "memory");
 }
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
 }
 
 // CTA (split, KV head, tile of 8 kNB packed rows)
@@ -498,6 +498,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (lane < kBuf) mbar_init(&sm.full[warp][lane], 1);
   fence_barrier_init();
   __syncwarp();
+  const bool cluster = sp.splits > 1 && !sp.partials;
+  if (cluster) cluster_arrive();  // waited for before anything is written to another CTA
   pdl_wait_then_release();  // launched with launch_pdl: nothing global is read before
   volatile int* abort = &sm.abort;
   const int kvh = blockIdx.y;
@@ -658,7 +660,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   const size_t tile = size_t(kvh) * gridDim.z + blockIdx.z;
   float* rec = sp.partials ? sp.partials + (tile * sp.splits + blockIdx.x) * kRecord : nullptr;
-  const bool cluster = sp.splits > 1 && !rec;
+  const int per_cta = (kRows + sp.splits - 1) / sp.splits;
+  if (cluster) cluster_wait();
   for (int idx = threadIdx.x; idx < n_rows * 32; idx += kThreads) {
     const int r = idx >> 5, d4 = idx & 31;
     float m = -INFINITY;
@@ -683,39 +686,41 @@ __global__ void __launch_bounds__(kThreads, 1)
       *reinterpret_cast<float4*>(rec + r * HD + 4 * d4) = acc;
       if (d4 == 0) reinterpret_cast<float2*>(rec + kMaxRows * HD)[r] = make_float2(m, l);
     } else if (cluster) {
-      // each element is read and written by this thread alone
-      *reinterpret_cast<float4*>(reinterpret_cast<float*>(sm.ring[0]) + r * (HD + 4) + 4 * d4) =
-          acc;
-      if (d4 == 0) sm.cta_ml[r] = make_float2(m, l);
+      const int to = r % sp.splits, at_row = int(blockIdx.x) * per_cta + r / sp.splits;
+      st_cluster_v4(cluster_addr(&sm.in_rows[at_row][d4], uint32_t(to)), acc);
+      if (d4 == 0) st_cluster_v2(cluster_addr(&sm.in_ml[at_row], uint32_t(to)), m, l);
     } else {
       store_row(p, kvh, row0 + r, d4, acc, m, l);
     }
   }
   if (!cluster) return;
-  // ---- join the cluster's CTAs: rows dealt out, each read from every CTA
-  cluster_sync();
-  for (int r = int(blockIdx.x) + sp.splits * warp; r < n_rows; r += sp.splits * kWarps) {
+  // ---- join the cluster's CTAs: rows dealt out, each now in its CTA's memory
+  cluster_arrive();
+  cluster_wait();
+  for (int i = warp; int(blockIdx.x) + sp.splits * i < n_rows; i += kWarps) {
+    float2 x[kMaxCluster];
     float m = -INFINITY;
-    for (int k = 0; k < sp.splits; ++k)
-      m = fmaxf(m, ld_cluster_v2(cluster_addr(&sm.cta_ml[r], uint32_t(k))).x);
+#pragma unroll
+    for (int k = 0; k < kMaxCluster; ++k) {
+      x[k] = k < sp.splits ? sm.in_ml[k * per_cta + i] : make_float2(-INFINITY, 0.f);
+      m = fmaxf(m, x[k].x);
+    }
     const float nm = m == -INFINITY ? 0.f : -m;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     float l = 0.f;
-#pragma unroll 4
-    for (int k = 0; k < sp.splits; ++k) {
-      const float2 x = ld_cluster_v2(cluster_addr(&sm.cta_ml[r], uint32_t(k)));
-      const float4 v = ld_cluster_v4(cluster_addr(
-          reinterpret_cast<const float*>(sm.ring[0]) + r * (HD + 4) + 4 * lane, uint32_t(k)));
-      const float f = ex2_approx(x.x + nm);
-      l += x.y * f;
+#pragma unroll
+    for (int k = 0; k < kMaxCluster; ++k) {
+      if (k >= sp.splits) break;
+      const float4 v = sm.in_rows[k * per_cta + i][lane];
+      const float f = ex2_approx(x[k].x + nm);
+      l += x[k].y * f;
       acc.x += v.x * f;
       acc.y += v.y * f;
       acc.z += v.z * f;
       acc.w += v.w * f;
     }
-    store_row(p, kvh, row0 + r, lane, acc, m, l);
+    store_row(p, kvh, row0 + int(blockIdx.x) + sp.splits * i, lane, acc, m, l);
   }
-  cluster_sync();  // no CTA leaves while another reads its rows
 }
 
 // Join the splits: CTA (packed row, KV head), its warps the splits in turn, lane
