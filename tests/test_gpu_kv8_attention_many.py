@@ -267,3 +267,44 @@ def test_refusals(dev):
             verify_attention_kv8(**{**ok, **change})
     out, lse = verify_attention_kv8(**ok)
     assert torch.isfinite(out).all() and torch.isfinite(lse).all()
+
+
+@pytest.mark.parametrize("q_len", [1, 5])
+@pytest.mark.parametrize("kv_len", [130, 600, 1100, 1600, 2100, 2600, 3100, 3600, 4100, 9000])
+def test_splits_of_few_rows(dev, q_len, kv_len):
+    """3 and 15 packed rows over ever more columns: one CTA, clusters of each size,
+    and more CTAs than a cluster holds."""
+    sealed = (kv_len - 40) // 64 * 64
+    allowed = T.segments([q_len], kv_len - q_len).to(dev)
+    x = T.make(dev, 6, 2, q_len, kv_len, sealed, seed=kv_len)
+    T.check(T.run(*x, sealed, T.plan_of(allowed)), T.exact(*x, sealed, allowed))
+
+
+@pytest.mark.parametrize("q_len", [3, 900])
+def test_plan_rebuilt_in_a_graph(dev, q_len):
+    """One graph builds the plan of a mask and attends in two layers right behind
+    it; replayed with other masks in the same memory."""
+    from hsd_b200.kv8 import Kv8Layer, verify_attention_kv8
+    from hsd_b200.plan import plan_from_dense
+    hq, hkv, kv_len, sealed = 12, 2, 2000, 1024
+    assert many(q_len, kv_len, hq, hkv) == (q_len == 900)
+    layers = [T.make(dev, hq, hkv, q_len, kv_len, sealed, seed=s) for s in (1, 2)]
+    g = torch.Generator().manual_seed(3)
+    masks, want = [], []
+    for density in (0.5, 0.02, 1.0, 0.0):
+        allowed = (torch.rand(q_len, kv_len, generator=g) < density).to(dev)
+        masks.append(torch.where(allowed, 0.0, -math.inf))
+        want.append([T.run(*x, sealed, T.plan_of(allowed)) for x in layers])
+    mask = masks[2].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        plan = plan_from_dense(mask)
+        got = [verify_attention_kv8(x[0], Kv8Layer(x[1][0], x[1][1], x[2][0], x[2][1]), sealed,
+                                    x[3][0], x[3][1], plan) for x in layers]
+    for i in (0, 1, 2, 3, 1, 0):
+        mask.copy_(masks[i])
+        graph.replay()
+        torch.cuda.synchronize()
+        plan.raise_on_device_error()
+        for (o, l), (wo, wl) in zip(got, want[i]):
+            assert torch.equal(o, wo) and torch.equal(l, wl)
