@@ -36,6 +36,8 @@ struct ExpandParams {
   const uint64_t* mask_words;
   uint16_t* dst;  // [2][hkv][kv_len][128]: K bf16, V fp16
   attn::ColumnScale* col_scale;
+  uint32_t* flags;  // of the attention, cleared here
+  int n_flags;
   int kv_len, hkv, n_kv64, n_qtiles, sealed, tail_row0;
   float scale_log2;
 };
@@ -83,6 +85,8 @@ __global__ void __launch_bounds__(kExpandThreads) expand_kernel(const ExpandPara
   pdl_wait_then_release();  // launched with launch_pdl
   __shared__ uint32_t red[2], warp_top[kExpandThreads / 32];
   const int t = blockIdx.x, h = blockIdx.y, z = blockIdx.z, tid = threadIdx.x;
+  if (t == 0 && h == 0 && z == 0)
+    for (int i = tid; i < p.n_flags; i += kExpandThreads) p.flags[i] = 0u;
   const int col0 = 64 * t;
   uint4* dst = reinterpret_cast<uint4*>(
       p.dst + (size_t(z * p.hkv + h) * p.kv_len + col0) * HD);
@@ -204,11 +208,12 @@ size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
 // Workspace of the path for many rows: flags, partial records, scales, rows.
 struct ManyLayout {
-  size_t scales, rows, total;
+  size_t partials, scales, rows, total;
 };
 ManyLayout many_layout(int32_t kv_len, int32_t hkv) {
   ManyLayout m;
-  m.scales = hsd_host::kKv8FlagBytes + align256(hsd_host::attention_partials_bytes());
+  m.partials = align256(hsd_host::attention_flags_bytes());
+  m.scales = m.partials + align256(hsd_host::attention_partials_bytes());
   m.rows = m.scales +
            align256(size_t(hkv) * ((kv_len + 127) / 128) * 2 * sizeof(hsd::attn::ColumnScale));
   m.total = m.rows + size_t(2) * hkv * kv_len * hsd::kv8a::HD * 2;
@@ -244,7 +249,7 @@ int many_launch(const hsd_host::Kv8AttnArgs& a, const hsd_plan_t& plan, float sc
   const kv8a::Params& p = a.p;
   int rc = hsd_host::attention_check_tiles(plan, "hsd_verify_attention_kv8");
   if (rc) return rc;
-  if (256 + hsd_host::attention_flags_bytes() > hsd_host::kKv8FlagBytes || p.hkv > 65535) {
+  if (p.hkv > 65535) {
     hsd_host::set_error("hsd_verify_attention_kv8: %d KV heads exceed the launch's range", p.hkv);
     return HSD_ERR_TOO_LARGE;
   }
@@ -268,6 +273,8 @@ int many_launch(const hsd_host::Kv8AttnArgs& a, const hsd_plan_t& plan, float sc
   e.mask_words = plan.mask_words;
   e.dst = reinterpret_cast<uint16_t*>(ws + m.rows);
   e.col_scale = reinterpret_cast<attn::ColumnScale*>(ws + m.scales);
+  e.flags = reinterpret_cast<uint32_t*>(ws);
+  e.n_flags = int(hsd_host::attention_flags_bytes() / sizeof(uint32_t));
   e.kv_len = p.kv_len;
   e.hkv = p.hkv;
   e.n_kv64 = p.n_kv64;
@@ -295,9 +302,9 @@ int many_launch(const hsd_host::Kv8AttnArgs& a, const hsd_plan_t& plan, float sc
   v.num_kv_heads = p.hkv;
   v.scale = scale;
   v.plan = &plan;
-  v.sync = reinterpret_cast<uint32_t*>(ws);
-  v.flags = reinterpret_cast<uint32_t*>(ws + 256);
-  v.partials = ws + hsd_host::kKv8FlagBytes;
+  v.sync = nullptr;
+  v.flags = e.flags;
+  v.partials = ws + m.partials;
   v.status = p.status;
   v.stream = reinterpret_cast<hsd_stream_t>(a.stream);
   v.col_scale = e.col_scale;

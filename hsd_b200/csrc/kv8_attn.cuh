@@ -64,10 +64,8 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
 }  // namespace hsd
 
 namespace hsd_host {
-// The two kernels behind hsd_verify_attention_kv8.  The workspace starts with
-// kKv8FlagBytes of flags and counters, zero before the first use and left
-// ready by every call; partial rows follow, in no state that a call relies on.
-constexpr size_t kKv8FlagBytes = 65536;
+// The two kernels behind hsd_verify_attention_kv8.  No call relies on what the
+// workspace holds when it starts.
 struct Kv8AttnArgs {
   hsd::kv8a::Params p;
   const int8_t* k8;

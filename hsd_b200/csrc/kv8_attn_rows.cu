@@ -907,9 +907,8 @@ Kv8RowsChoice kv8_rows_choose(int q_len, int kv_len, int hq, int hkv) {
 }
 
 size_t kv8_rows_workspace_bytes(int q_len, int hq, int hkv, int splits) {
-  if (splits <= kv8r::kMaxCluster) return kKv8FlagBytes;
-  return kKv8FlagBytes +
-         size_t(n_tiles(q_len, hq / hkv)) * hkv * splits * kv8r::kRecord * sizeof(float);
+  if (splits <= kv8r::kMaxCluster) return 256;  // nothing, but a workspace all the same
+  return size_t(n_tiles(q_len, hq / hkv)) * hkv * splits * kv8r::kRecord * sizeof(float);
 }
 
 int kv8_map(CUtensorMap* map, const void* base, bool bf16, int64_t rows, int heads,
@@ -969,7 +968,7 @@ int kv8_rows_launch(const Kv8AttnArgs& a, int splits) {
   sp.splits = splits;
   const bool cluster = sp.splits > 1 && sp.splits <= kv8r::kMaxCluster;
   sp.partials = sp.splits > kv8r::kMaxCluster
-                    ? reinterpret_cast<float*>(static_cast<char*>(a.workspace) + kKv8FlagBytes)
+                    ? static_cast<float*>(a.workspace)
                     : nullptr;
   if (sp.n_tiles > 65535 || p.hkv > 65535) {
     set_error("hsd_verify_attention_kv8: %d rows x %d heads exceed the launch's range", p.q_len,

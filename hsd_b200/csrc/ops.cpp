@@ -357,26 +357,19 @@ Heads heads_of(const Args& a, const at::Tensor& t, const char* name) {
   return h;
 }
 
-constexpr int64_t kFlagBytes = 65536;  // leading part of the workspace that starts as zeros
-
-// Scratch of (device, current stream), grown to fit; its flags are zeroed once
-// and every call leaves them ready for the next.  A call that is being captured
-// into a graph gets scratch of its own, zeroed by the graph, so graphs that
-// share no stream share no scratch either (replays of one graph never overlap).
+// Scratch of (device, current stream), grown to fit.  A call that is being captured
+// into a graph gets scratch of its own from the graph's pool, so graphs that share
+// no stream share no scratch either (replays of one graph never overlap).
 at::Tensor workspace(int64_t need, const c10::Device& dev) {
   const auto opt = at::TensorOptions().dtype(at::kByte).device(dev);
-  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) {
-    at::Tensor t = at::empty({need + 256}, opt);
-    t.narrow(0, 0, kFlagBytes + 256).zero_();
-    return t;
-  }
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
+    return at::empty({need + 256}, opt);
   // never destroyed: tensors must not outlive the allocator at exit
   static auto* cached = new std::map<std::pair<int, void*>, at::Tensor>;
   at::Tensor& t = (*cached)[{dev.index(), c10::cuda::getCurrentCUDAStream(dev.index()).stream()}];
   if (!t.defined() || t.numel() < need + 256) {
     t = at::Tensor();
     t = at::empty({std::max<int64_t>(need, 1 << 20) + 256}, opt);
-    t.narrow(0, 0, kFlagBytes + 256).zero_();
   }
   return t;
 }

@@ -322,7 +322,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* abort = &sm.abort;
   const int total = p.blk_prefix[p.n_qtiles] * per_tile;
   const int G = gridDim.x;
-  const uint32_t gen = p.split ? __ldcg(p.sync) : 0u;  // launch generation (stream-K flags)
+  // launch generation (stream-K flags); kScaled: the expansion has cleared the flags
+  const uint32_t gen = p.split && !kScaled ? __ldcg(p.sync) : 0u;
   int w0, w1;
   if (p.split) {
     w0 = range_start(blockIdx.x, total, G);
@@ -971,7 +972,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if constexpr (kScaled) asm volatile("griddepcontrol.wait;" ::: "memory");
   tc_fence_before();
   __syncthreads();
-  if (p.split && threadIdx.x == 0) {
+  if (!kScaled && p.split && threadIdx.x == 0) {
     // the last CTA to finish advances the generation for the next launch
     __threadfence();
     if (atomicAdd(p.sync + 1, 1u) == uint32_t(G) - 1u) {

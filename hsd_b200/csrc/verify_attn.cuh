@@ -23,7 +23,8 @@ namespace hsd_host {
 // Checked arguments of hsd_verify_attention; partials, flags and sync are the
 // stream-K scratch (all null: one CTA per item); with
 // col_scale [num_kv_heads][2 ceil(kv_len / 128)], k (bf16) and v (fp16) hold values
-// that the scales multiply, and `scale` is not used.
+// that the scales multiply, `scale` and sync are not used, and the kernel launched
+// just before, which has waited for all before it, clears the flags.
 struct AttentionArgs {
   const void *q, *k, *v;
   int64_t q_row_stride, q_head_stride, k_row_stride, k_head_stride, v_row_stride, v_head_stride;

@@ -401,10 +401,8 @@ int hsd_kv8_unseal(const int8_t *data, int64_t plane_stride, const float *scale,
  * Two paths by size: few rows read the cache as it is; many first expand the
  * layer's columns into the workspace, which then holds 512 bytes per column
  * and KV head.
- * workspace: hsd_kv8_attention_workspace_bytes, 256-byte aligned, its first
- * 64 KB zero-filled before the first use; each call leaves it ready for the
- * next (after an error status, zero them again), and calls sharing one must
- * not overlap in time. */
+ * workspace: hsd_kv8_attention_workspace_bytes, 256-byte aligned, with any
+ * contents; calls sharing one must not overlap in time. */
 size_t hsd_kv8_attention_workspace_bytes(int32_t q_len, int32_t kv_len, int32_t num_q_heads,
                                          int32_t num_kv_heads);
 int hsd_verify_attention_kv8(const void *q, int64_t q_row_stride, int64_t q_head_stride,
