@@ -12,8 +12,8 @@
 // P can be fp16 and keep 11 bits.  The expansion reads 1 byte and writes 2 per
 // sealed value, and the attention finds it in L2; for a region step's 4800 columns of
 // 2 heads it is latency (7.1 us alone from cold caches, about 3.5 in a stream of steps,
-// where the attention's setup runs under it).  Both together: 53.2 us for 2176 rows,
-// 12/2 heads, 4800 columns (the bf16 kernel alone 47.8), 217 us for 2049 rows and
+// where the attention's setup runs under it).  Both together: 51.7 us for 2176 rows,
+// 12/2 heads, 4800 columns (the bf16 kernel alone 47.8), 215 us for 2049 rows and
 // 18,450 columns (210).
 #include "kv8_attn.cuh"
 #include "verify_attn.cuh"
@@ -220,13 +220,13 @@ ManyLayout many_layout(int32_t kv_len, int32_t hkv) {
   return m;
 }
 
-// Rows kernel or many rows, by the time each takes.  Many rows: 24 us, the expansion
+// Rows kernel or many rows, by the time each takes.  Many rows: 22 us, the expansion
 // (1.3e-4 us a column and KV head), 2.05 us per SM for every 128 rows x 128 columns x
 // two heads, and 1.2 us for each part of an item (128 rows, two heads) that its first
 // CTA merges when all SMs share few items.  Measured (rows / many, us): 12/2 heads, 1600
-// columns: 128 rows 18 / 38, 256 rows 37 / 38, 384 rows 36 / 32; 8192 columns: 64 rows
-// 36 / 60, 128 rows 58 / 60, 256 rows 101 / 50; 16/8 heads, 32768 columns: 32 rows 62 /
-// 113, 128 rows 207 / 113; 8/1 heads, 32768 columns: 64 rows 62 / 88, 128 rows 111 / 88.
+// columns: 128 rows 17 / 36, 256 rows 37 / 36, 384 rows 35 / 30; 8192 columns: 64 rows
+// 34 / 58, 128 rows 57 / 58, 256 rows 99 / 48; 16/8 heads, 32768 columns: 32 rows 60 /
+// 111, 128 rows 206 / 111; 8/1 heads, 32768 columns: 64 rows 60 / 88, 128 rows 110 / 88.
 struct Path {
   int splits;  // rows kernel: CTAs per tile; 0: many rows
   size_t bytes;
@@ -237,7 +237,7 @@ Path choose_path(int32_t q_len, int32_t kv_len, int32_t hq, int32_t hkv) {
   const float items = float((q_len + 127) / 128) * float((hq / hkv + 1) / 2) * float(hkv);
   const float blocks = float((kv_len + 127) / 128);
   const float merges = std::max(std::min(blocks, sms / items) - 1.f, 0.f);
-  const float many = 24.f + 1.3e-4f * float(kv_len) * float(hkv) +
+  const float many = 22.f + 1.3e-4f * float(kv_len) * float(hkv) +
                      2.05f * items * blocks / sms + 1.2f * merges;
   if (rows.us <= many)
     return {rows.splits, hsd_host::kv8_rows_workspace_bytes(q_len, hq, hkv, rows.splits)};

@@ -34,14 +34,13 @@
 // fp32; the row sum takes the unrounded P.
 //
 // Measured: one row, 16/8 heads, 131,051 columns (269 MB): 47 us and 4 us for the
-// join, 5.1 TB/s over both (0.79 of a copy; a wait of 3 to 4 us for the first tiles
-// and the join are what is left).  12/2 heads, 2625 columns: one row 7.7 us, forty
-// 13.2 us: latency (launch, block list, tile, join), not bytes.
+// join, 5.3 TB/s over both (0.82 of a copy; a wait of 3 to 4 us for the first tiles
+// and the join are what is left).  12/2 heads, 2625 columns: one row 6.0 us, forty
+// 11.7 us: latency (launch, block list, tile, join), not bytes.
 //
 // Join: warps of a CTA through shared memory; up to eight CTAs of a tile as a
 // cluster, each writing its rows into the shared memory of the CTA that joins them
-// (reading them from there instead took a second barrier: one row 8.5 us for
-// 7.7); more through fp32 partial rows in the workspace and a second small
+// (reading them from there instead took a second barrier and 0.8 us); more through fp32 partial rows in the workspace and a second small
 // launch.  No counters
 // and no flags: the result does not depend on the order in which CTAs finish.
 #include "kv8_attn.cuh"
