@@ -225,10 +225,11 @@ ManyLayout many_layout(int32_t kv_len, int32_t hkv) {
 // two heads, and 1.2 us for each part of an item (128 rows, two heads) that its first
 // CTA merges when all SMs share few items.  Measured (rows / many, us): 12/2 heads, 1600
 // columns: 128 rows 17 / 36, 256 rows 37 / 36, 384 rows 35 / 30; 8192 columns: 64 rows
-// 34 / 58, 128 rows 57 / 58, 256 rows 99 / 48; 16/8 heads, 32768 columns: 32 rows 60 /
+// 27 / 58, 128 rows 57 / 58, 256 rows 99 / 48; 16/8 heads, 32768 columns: 32 rows 60 /
 // 111, 128 rows 206 / 111; 8/1 heads, 32768 columns: 64 rows 60 / 88, 128 rows 110 / 88.
 struct Path {
-  int splits;  // rows kernel: CTAs per tile; 0: many rows
+  bool many;
+  hsd_host::Kv8RowsChoice rows;
   size_t bytes;
 };
 Path choose_path(int32_t q_len, int32_t kv_len, int32_t hq, int32_t hkv) {
@@ -240,8 +241,8 @@ Path choose_path(int32_t q_len, int32_t kv_len, int32_t hq, int32_t hkv) {
   const float many = 22.f + 1.3e-4f * float(kv_len) * float(hkv) +
                      2.05f * items * blocks / sms + 1.2f * merges;
   if (rows.us <= many)
-    return {rows.splits, hsd_host::kv8_rows_workspace_bytes(q_len, hq, hkv, rows.splits)};
-  return {0, many_layout(kv_len, hkv).total};
+    return {false, rows, hsd_host::kv8_rows_workspace_bytes(q_len, hq, hkv, rows)};
+  return {true, rows, many_layout(kv_len, hkv).total};
 }
 
 int many_launch(const hsd_host::Kv8AttnArgs& a, const hsd_plan_t& plan, float scale) {
@@ -409,5 +410,5 @@ extern "C" int hsd_verify_attention_kv8(
   a.vt_head_stride = vt_head_stride;
   a.workspace = workspace;
   a.stream = reinterpret_cast<cudaStream_t>(stream);
-  return path.splits ? hsd_host::kv8_rows_launch(a, path.splits) : many_launch(a, *plan, scale);
+  return path.many ? many_launch(a, *plan, scale) : hsd_host::kv8_rows_launch(a, path.rows);
 }

@@ -77,16 +77,17 @@ struct Kv8AttnArgs {
   void* workspace;
   cudaStream_t stream;
 };
-// CTAs per tile of the rows kernel for these sizes, its time by its own model, and
-// the device's SMs.
+// The rows kernel for these sizes: CTAs per tile, whether the join kernel joins them
+// (else they are a cluster), its time by its own model, and the device's SMs.
 struct Kv8RowsChoice {
   int splits;
+  bool join;
   float us;
   int sms;
 };
 Kv8RowsChoice kv8_rows_choose(int q_len, int kv_len, int hq, int hkv);
-size_t kv8_rows_workspace_bytes(int q_len, int hq, int hkv, int splits);
-int kv8_rows_launch(const Kv8AttnArgs& a, int splits);
+size_t kv8_rows_workspace_bytes(int q_len, int hq, int hkv, const Kv8RowsChoice& c);
+int kv8_rows_launch(const Kv8AttnArgs& a, const Kv8RowsChoice& c);
 // 3-D map {128 dims, rows, heads} of int8 (box 128 x box_rows) or bf16 (box
 // 64 x box_rows), 128-byte swizzle.
 int kv8_map(CUtensorMap* map, const void* base, bool bf16, int64_t rows, int heads,

@@ -38,11 +38,11 @@
 // and the join are what is left).  12/2 heads, 2625 columns: one row 6.0 us, forty
 // 11.7 us: latency (launch, block list, tile, join), not bytes.
 //
-// Join: warps of a CTA through shared memory; up to eight CTAs of a tile as a
+// Join: warps of a CTA through shared memory; up to sixteen CTAs of a tile as a
 // cluster, each writing its rows into the shared memory of the CTA that joins them
-// (reading them from there instead took a second barrier and 0.8 us); more through fp32 partial rows in the workspace and a second small
-// launch.  No counters
-// and no flags: the result does not depend on the order in which CTAs finish.
+// (reading them from there instead took a second barrier and 0.8 us); or, where
+// clusters do not fit, through fp32 partial rows in the workspace and a second small
+// launch.  No counters and no flags: the result does not depend on the order in which CTAs finish.
 #include "kv8_attn.cuh"
 
 #include <algorithm>
@@ -65,8 +65,8 @@ constexpr int kBuf = 3;  // the issue order keeps exactly three tiles ahead
 static_assert(kBuf == 3, "a step's K and V and the next step's K are issued before any is used");
 constexpr int kRing = kBuf * kTile;  // a warp's buffers: K, V, K, V, ... in turn
 constexpr int kMaxRows = 16;
-constexpr int kMaxCluster = 8;
-constexpr int kMaxIn = 21;  // the most of s ceil(kMaxRows / s) for s <= kMaxCluster
+constexpr int kMaxCluster = 16;  // above 8: by opt-in, where the device has room for them
+constexpr int kMaxIn = 30;  // the most of s ceil(kMaxRows / s) for s <= kMaxCluster
 constexpr int kRecord = kMaxRows * HD + 2 * kMaxRows;  // floats of a partial record
 constexpr float kPShift = 15.0f;                 // P = 2^15 exp(s - max)
 
@@ -810,10 +810,14 @@ auto rows_kernel_of(bool wide) { return wide ? kv8r::rows_kernel<2> : kv8r::rows
 
 int set_rows_attribute(bool wide, int dev) {
   if (g_attr_set[wide][dev].load(std::memory_order_acquire)) return HSD_OK;
-  const int rc = cuda_check(
+  int rc = cuda_check(
       cudaFuncSetAttribute(rows_kernel_of(wide), cudaFuncAttributeMaxDynamicSharedMemorySize,
                            int(kv8r::kSmem)),
       "cudaFuncSetAttribute(rows_kernel)");
+  if (rc == HSD_OK)
+    rc = cuda_check(cudaFuncSetAttribute(rows_kernel_of(wide),
+                                         cudaFuncAttributeNonPortableClusterSizeAllowed, 1),
+                    "cudaFuncSetAttribute(rows_kernel)");
   if (rc == HSD_OK) g_attr_set[wide][dev].store(true, std::memory_order_release);
   return rc;
 }
@@ -830,10 +834,11 @@ struct Device {
   int clusters[2][kv8r::kMaxCluster + 1];  // [16 rows][CTAs of a cluster]
 };
 
-// Clusters of s CTAs at once: SMs of a cluster lie in one group of the chip, so
-// this is less than SMs / s.
+// Clusters of s CTAs at once, 0 if none: SMs of a cluster lie in one group of the
+// chip, so this is less than SMs / s.
 int resident_clusters(bool wide, int s, int dev, int sms) {
-  if (s == 1 || set_rows_attribute(wide, dev) != HSD_OK) return sms / s;
+  if (s == 1) return sms;
+  if (set_rows_attribute(wide, dev) != HSD_OK) return 0;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(s * sms));
   cfg.blockDim = dim3(kv8r::kThreads);
@@ -845,9 +850,7 @@ int resident_clusters(bool wide, int s, int dev, int sms) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   int n = 0;
-  return cudaOccupancyMaxActiveClusters(&n, rows_kernel_of(wide), &cfg) == cudaSuccess && n > 0
-             ? n
-             : sms / s;
+  return cudaOccupancyMaxActiveClusters(&n, rows_kernel_of(wide), &cfg) == cudaSuccess ? n : 0;
 }
 
 const Device& current_device() {
@@ -867,17 +870,18 @@ const Device& current_device() {
     for (int wide = 0; wide < 2; ++wide)
       for (int s = 1; s <= kv8r::kMaxCluster; ++s)
         d.clusters[wide][s] =
-            dev < kMaxDevices ? resident_clusters(wide, s, dev, d.sms) : d.sms / s;
+            dev < kMaxDevices ? resident_clusters(wide, s, dev, d.sms) : 0;
     cudaGetLastError();
   });
   return table[dev];
 }
 
-// CTAs per tile and what the launch then takes.  With every SM busy a warp's step
-// takes about 3.3 us (16 rows; 2 us for 8) and a CTA 5 us besides (measured at 1600
-// to 32768 columns), so the time goes by the waves of clusters and the steps of a
-// warp; more than kMaxCluster CTAs per tile, when there are few tiles, need the
-// join kernel (4 us).
+// CTAs per tile and what the launch then takes.  A launch takes about 4.2 us (16 rows
+// a tile: 5.2) and 2.7 us (3.4) for each step of a warp, so the time goes by the waves
+// of clusters and the steps; the join kernel (2 us) lets CTAs be dealt out
+// without regard to clusters, or more than kMaxCluster of them to a tile.  Measured, 12/2 heads, one row: 4097 columns 6.8
+// us with a cluster of 9 (of 8: 9.4), 12,001 columns 9.2 with 12 (9.6 to 12 with 8), 16,385
+// columns 8.3 with 33 CTAs and the join (cluster of 16: 12.1).
 Kv8RowsChoice choose(int q_len, int kv_len, int hq, int hkv) {
   const Device& dev = current_device();
   const int64_t tiles = int64_t(n_tiles(q_len, hq / hkv)) * hkv;
@@ -886,17 +890,18 @@ Kv8RowsChoice choose(int q_len, int kv_len, int hq, int hkv) {
   const int most = (units + kv8r::kWarps - 1) / kv8r::kWarps;
   auto time = [&](int64_t waves, int s) {
     const int steps = (units + s * kv8r::kWarps - 1) / (s * kv8r::kWarps);
-    return float(waves) * (5.f + (wide ? 3.3f : 2.f) * float(steps));
+    return float(waves) * (wide ? 5.2f + 3.4f * float(steps) : 4.2f + 2.7f * float(steps));
   };
-  Kv8RowsChoice best{1, time((tiles + dev.sms - 1) / dev.sms, 1), dev.sms};
+  Kv8RowsChoice best{1, false, time((tiles + dev.sms - 1) / dev.sms, 1), dev.sms};
   for (int s = 2; s <= kv8r::kMaxCluster && s <= most; ++s) {
     const int at_once = dev.clusters[wide][s];
+    if (at_once < 1) continue;
     const float us = time((tiles + at_once - 1) / at_once, s);
-    if (us < best.us) best = {s, us, dev.sms};
+    if (us < best.us) best = {s, false, us, dev.sms};
   }
   const int64_t s = std::min<int64_t>(dev.sms / tiles, most);
-  if (s > kv8r::kMaxCluster && time(1, int(s)) + 4.f < best.us)
-    best = {int(s), time(1, int(s)) + 4.f, dev.sms};
+  if (s > 1 && time(1, int(s)) + 2.f < best.us)
+    best = {int(s), true, time(1, int(s)) + 2.f, dev.sms};
   return best;
 }
 }  // namespace
@@ -905,9 +910,9 @@ Kv8RowsChoice kv8_rows_choose(int q_len, int kv_len, int hq, int hkv) {
   return choose(q_len, kv_len, hq, hkv);
 }
 
-size_t kv8_rows_workspace_bytes(int q_len, int hq, int hkv, int splits) {
-  if (splits <= kv8r::kMaxCluster) return 256;  // nothing, but a workspace all the same
-  return size_t(n_tiles(q_len, hq / hkv)) * hkv * splits * kv8r::kRecord * sizeof(float);
+size_t kv8_rows_workspace_bytes(int q_len, int hq, int hkv, const Kv8RowsChoice& c) {
+  if (!c.join) return 256;  // nothing, but a workspace all the same
+  return size_t(n_tiles(q_len, hq / hkv)) * hkv * c.splits * kv8r::kRecord * sizeof(float);
 }
 
 int kv8_map(CUtensorMap* map, const void* base, bool bf16, int64_t rows, int heads,
@@ -934,7 +939,7 @@ int kv8_map(CUtensorMap* map, const void* base, bool bf16, int64_t rows, int hea
   return HSD_OK;
 }
 
-int kv8_rows_launch(const Kv8AttnArgs& a, int splits) {
+int kv8_rows_launch(const Kv8AttnArgs& a, const Kv8RowsChoice& c) {
   const hsd::kv8a::Params& p = a.p;
   CUtensorMap k8, v8, kt, vt;
   const int64_t tail_rows = p.kv_len - p.tail_row0;
@@ -964,11 +969,8 @@ int kv8_rows_launch(const Kv8AttnArgs& a, int splits) {
   kv8r::Split sp;
   sp.n_tiles = n_tiles(p.q_len, p.group);
   sp.rows = tile_rows(p.q_len, p.group);
-  sp.splits = splits;
-  const bool cluster = sp.splits > 1 && sp.splits <= kv8r::kMaxCluster;
-  sp.partials = sp.splits > kv8r::kMaxCluster
-                    ? static_cast<float*>(a.workspace)
-                    : nullptr;
+  sp.splits = c.splits;
+  sp.partials = c.join ? static_cast<float*>(a.workspace) : nullptr;
   if (sp.n_tiles > 65535 || p.hkv > 65535) {
     set_error("hsd_verify_attention_kv8: %d rows x %d heads exceed the launch's range", p.q_len,
               p.hq);
@@ -987,7 +989,7 @@ int kv8_rows_launch(const Kv8AttnArgs& a, int splits) {
   rc = launch_pdl(rows_kernel_of(wide),
                   dim3(unsigned(sp.splits), unsigned(p.hkv), unsigned(sp.n_tiles)),
                   dim3(kv8r::kThreads), kv8r::kSmem, a.stream, "rows_kernel launch",
-                  cluster ? unsigned(sp.splits) : 0u, k8, v8, kt, vt, p, sp);
+                  c.splits > 1 && !c.join ? unsigned(c.splits) : 0u, k8, v8, kt, vt, p, sp);
   if (rc || !sp.partials) return rc;
   return launch_pdl(kv8r::join_kernel,
                     dim3(unsigned(p.q_len * p.group), unsigned(p.hkv)),
