@@ -878,10 +878,11 @@ const Device& current_device() {
 
 // CTAs per tile and what the launch then takes.  A launch takes about 4.2 us (16 rows
 // a tile: 5.2) and 2.7 us (3.4) for each step of a warp, so the time goes by the waves
-// of clusters and the steps; the join kernel (2 us) lets CTAs be dealt out
-// without regard to clusters, or more than kMaxCluster of them to a tile.  Measured, 12/2 heads, one row: 4097 columns 6.8
-// us with a cluster of 9 (of 8: 9.4), 12,001 columns 9.2 with 12 (9.6 to 12 with 8), 16,385
-// columns 8.3 with 33 CTAs and the join (cluster of 16: 12.1).
+// of clusters and the steps; the join kernel (2 us) lets CTAs be dealt out without
+// regard to clusters, or more than kMaxCluster of them to a tile.  Measured, 12/2
+// heads, one row: 4097 columns 6.7 us with a cluster of 9 (of 8: 9.4), 8193 columns 7.9
+// with 17 CTAs and the join (cluster of 16: 9.6, of 8: 12.0), 16,385 columns 8.1 with 33
+// (cluster of 16: 12.1).
 Kv8RowsChoice choose(int q_len, int kv_len, int hq, int hkv) {
   const Device& dev = current_device();
   const int64_t tiles = int64_t(n_tiles(q_len, hq / hkv)) * hkv;
