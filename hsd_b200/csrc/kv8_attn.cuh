@@ -82,6 +82,7 @@ struct Kv8AttnArgs {
 struct Kv8RowsChoice {
   int splits;
   bool join;
+  bool fine;  // sealed columns 32 at a time instead of 64
   float us;
   int sms;
 };

@@ -4,10 +4,10 @@
 // What bounds it is reading the cache once, so the rows of all query heads of
 // one KV head are packed (packed row i = query row i / group, head i % group)
 // into tiles of 16, and the cache's columns are split over all SMs.  A warp
-// owns a running softmax of one tile and takes 64 sealed columns (or 32 bf16
-// ones) at a time: one TMA copy each of K and V, 8 KB each, into its own three
-// buffers, each refilled as soon as its tile has been used; no warp waits for
-// another before the join.  At full rate a copy takes 3 to 4 us, so the SM needs
+// owns a running softmax of one tile and takes 64 sealed columns (32 where that
+// leaves each warp one step; 32 bf16 ones) at a time: one TMA copy each of K and V,
+// 8 KB each, into its own three buffers, each refilled as soon as its tile has been
+// used; no warp waits for another before the join.  At full rate a copy takes 3 to 4 us, so the SM needs
 // about 150 KB in flight: eight warps with three tiles each (with two tiles a
 // warp waited 870 of 6300 cycles for V).
 //
@@ -35,7 +35,7 @@
 //
 // Measured: one row, 16/8 heads, 131,051 columns (269 MB): 47 us and 4 us for the
 // join, 5.3 TB/s over both (0.82 of a copy; a wait of 3 to 4 us for the first tiles
-// and the join are what is left).  12/2 heads, 2625 columns: one row 6.0 us, forty
+// and the join are what is left).  12/2 heads, 2625 columns: one row 5.3 us, forty
 // 11.7 us: latency (launch, block list, tile, join), not bytes.
 //
 // Join: warps of a CTA through shared memory; up to sixteen CTAs of a tile as a
@@ -112,8 +112,9 @@ __device__ __forceinline__ uint4 lds128(const uint8_t* p) {
   return *reinterpret_cast<const uint4*>(p);
 }
 
-// The warp's walk over its units: 64-column halves of the tile's block list,
-// a bf16 half in two steps of 32 columns.  The list is read a unit ahead.
+// The warp's walk over its units: 64-column halves of the tile's block list (a bf16
+// half in two steps of 32 columns), or, NT = 2, 32-column quarters.  The list is read
+// a unit ahead.
 struct Walk {
   const uint32_t* list;
   int n_units, stride, u;
@@ -125,14 +126,17 @@ struct Step {
   bool tail, second, partial;
 };
 
+template <int NT>
 __device__ __forceinline__ uint32_t list_entry(const Walk& w, int u) {
   // does not wait for n_units; next_step ignores what lies behind it
-  return (u >> 1) < w.room ? w.list[u >> 1] : 0u;
+  const int i = u >> (NT == 4 ? 1 : 2);
+  return i < w.room ? w.list[i] : 0u;
 }
 
+template <int NT>
 __device__ __forceinline__ Step next_step(const Params& p, Walk& w, const Step& last) {
   Step c;
-  if (last.col >= 0 && last.tail && !last.second && last.col + 32 < p.kv_len) {
+  if (NT == 4 && last.col >= 0 && last.tail && !last.second && last.col + 32 < p.kv_len) {
     c = last;
     c.second = true;
     c.col += 32;
@@ -148,11 +152,19 @@ __device__ __forceinline__ Step next_step(const Params& p, Walk& w, const Step& 
       return c;
     }
     w.u += w.stride;
-    w.ahead = list_entry(w, w.u);
-    const int hf = u & 1;
+    w.ahead = list_entry<NT>(w, w.u);
+    const int hf = (NT == 4 ? u : u >> 1) & 1;
     if (!((e >> (24 + 2 * hf)) & 1u)) continue;
     c.partial = ((e >> (25 + 2 * hf)) & 1u) != 0;
     c.col = int(e & 0xFFFFFFu) * 128 + 64 * hf;
+    if (NT == 2 && (u & 1)) {
+      c.second = true;
+      c.col += 32;
+      if (c.col >= p.kv_len) {
+        c.second = false;
+        continue;
+      }
+    }
     c.tail = c.col >= p.sealed;
     return c;
   }
@@ -275,21 +287,21 @@ __device__ __forceinline__ void softmax_step(float (&c)[kNB][NT][4],
   }
 }
 
-template <int kNB>
+template <int kNB, int NT>
 __device__ __forceinline__ void sealed_scores(const uint8_t* kb, const uint2 (*q16)[2][32], int g,
-                                              int t, float (&c)[kNB][4][4]) {
+                                              int t, float (&c)[kNB][NT][4]) {
   const int pg = perm(g), lane = lane_id();
 #pragma unroll
   for (int b = 0; b < kNB; ++b)
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) c[b][j][i] = 0.f;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    uint32_t w[8][4];  // column perm(g) of eight times eight
+    uint32_t w[2 * NT][4];  // column perm(g) of every eight
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < 2 * NT; ++j) {
       const uint4 v = lds128(kb + (8 * j + pg) * 128 + (((4 * h + t) ^ pg) << 4));
       w[j][0] = v.x;
       w[j][1] = v.y;
@@ -302,7 +314,7 @@ __device__ __forceinline__ void sealed_scores(const uint8_t* kb, const uint2 (*q
 #pragma unroll
       for (int b = 0; b < kNB; ++b) q[b] = q16[4 * h + k][b][lane];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < NT; ++j) {
         uint32_t a[4];
         bytes_to_f16(w[2 * j][k], a[0], a[2]);
         bytes_to_f16(w[2 * j + 1][k], a[1], a[3]);
@@ -313,12 +325,12 @@ __device__ __forceinline__ void sealed_scores(const uint8_t* kb, const uint2 (*q
   }
 }
 
-template <int kNB>
-__device__ __forceinline__ void sealed_values(const uint8_t* vb, const uint32_t (&pk)[kNB][4][2],
+template <int kNB, int NT>
+__device__ __forceinline__ void sealed_values(const uint8_t* vb, const uint32_t (&pk)[kNB][NT][2],
                                               int g, int t, State<kNB>& s) {
   const int pg = perm(g);
 #pragma unroll
-  for (int kk = 0; kk < 4; ++kk) {
+  for (int kk = 0; kk < NT; ++kk) {
     uint32_t w[4][4];  // rows t, t + 4, t + 8, t + 12 of the 16: dims 16 pg..+15
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -481,8 +493,8 @@ __device__ __forceinline__ void cluster_wait() {
   asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
 }
 
-// CTA (split, KV head, tile of 8 kNB packed rows)
-template <int kNB>
+// CTA (split, KV head, tile of 8 kNB packed rows); sealed steps of 16 NT columns
+template <int kNB, int NT>
 __global__ void __launch_bounds__(kThreads, 1)
     rows_kernel(const __grid_constant__ CUtensorMap tm_k8,
                 const __grid_constant__ CUtensorMap tm_v8,
@@ -510,11 +522,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint4 q_dims = load_q(p, kvh, row0, n_rows);
   Walk walk;
   walk.list = p.blk_list + size_t(qt) * p.n_kv128;
-  walk.n_units = 2 * p.blk_count[qt];
+  walk.n_units = (NT == 4 ? 2 : 4) * p.blk_count[qt];
   walk.room = p.n_kv128;
   walk.stride = sp.splits * kWarps;
   walk.u = int(blockIdx.x) * kWarps + warp;
-  walk.ahead = list_entry(walk, walk.u);
+  walk.ahead = list_entry<NT>(walk, walk.u);
   uint8_t* ring = sm.ring[warp];
   // operand tile i (K of step n: 2 n, V: 2 n + 1) into buffer i % kBuf
   int issued = 0;
@@ -523,7 +535,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) {
       uint64_t* bar = &sm.full[warp][fill];
       uint8_t* dst = ring + fill * kTile;
-      mbar_arrive_expect_tx(bar, kTile);
+      mbar_arrive_expect_tx(bar, c.tail ? kTile : 16 * NT * HD);
       if (c.tail) {
         for (int h = 0; h < 2; ++h)
           tma_load_3d(dst + h * (kTile / 2), is_v ? &tm_vt : &tm_kt, bar, 64 * h,
@@ -538,7 +550,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   Step none;
   none.col = -1;
   none.tail = none.second = none.partial = false;
-  Step cur = next_step(p, walk, none);
+  Step cur = next_step<NT>(p, walk, none);
   if (cur.col >= 0) {
     issue(cur, false);
     issue(cur, true);
@@ -553,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (cur.col >= 0) load_aside<kNB>(p, cur, kvh, qt, mrow, a);
   stage_q<kNB>(sm, q_dims);
   Step nxt = none;
-  if (cur.col >= 0) nxt = next_step(p, walk, cur);
+  if (cur.col >= 0) nxt = next_step<NT>(p, walk, cur);
   if (nxt.col >= 0) issue(nxt, false);
   __syncthreads();  // Q fragments and the abort word
 
@@ -591,14 +603,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
   while (cur.col >= 0) {
     Step after = none;  // the step after next
-    if (nxt.col >= 0) after = next_step(p, walk, nxt);
+    if (nxt.col >= 0) after = next_step<NT>(p, walk, nxt);
     uint64_t all = ~0ull, some = 0ull;
 #pragma unroll
     for (int r = 0; r < 2 * kNB; ++r) {
       all &= a.bits[r];
       if (mrow[r] >= 0) some |= a.bits[r];
     }
-    if (cur.tail) all |= 0xffffffff00000000ull;
+    if (NT == 2 || cur.tail) all |= 0xffffffff00000000ull;
     const bool masked = __any_sync(0xffffffffu, all != ~0ull);
     const bool any = !masked || __any_sync(0xffffffffu, some != 0ull);
     if (!wait_tile(0x800)) break;
@@ -619,18 +631,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!wait_tile(0x801)) break;
       if (any) tail_values<kNB>(ring + at * kTile, pk, seen, g, t, s);
     } else {
-      float c[kNB][4][4];
-      sealed_scores<kNB>(ring + at * kTile, sm.q16, g, t, c);
+      float c[kNB][NT][4];
+      sealed_scores<kNB, NT>(ring + at * kTile, sm.q16, g, t, c);
       done_tile();
       if (nxt.col >= 0) issue(nxt, true);
-      uint32_t pk[kNB][4][2];
+      uint32_t pk[kNB][NT][2];
       float sc[2 * kNB];
 #pragma unroll
       for (int r = 0; r < 2 * kNB; ++r) sc[r] = a.ks * q_unit[r];
-      if (any) softmax_step<kNB, 4, true>(c, a.bits, masked, sc, a.vs, pg, s, pk);
+      if (any) softmax_step<kNB, NT, true>(c, a.bits, masked, sc, a.vs, pg, s, pk);
       if (nxt.col >= 0) load_aside<kNB>(p, nxt, kvh, qt, mrow, a);
       if (!wait_tile(0x802)) break;
-      if (any) sealed_values<kNB>(ring + at * kTile, pk, g, t, s);
+      if (any) sealed_values<kNB, NT>(ring + at * kTile, pk, g, t, s);
     }
     done_tile();
     if (after.col >= 0) issue(after, false);
@@ -804,21 +816,24 @@ using namespace hsd;
 
 namespace {
 constexpr int kMaxDevices = 64;
-std::atomic<bool> g_attr_set[2][kMaxDevices];  // [16 rows][device]
+std::atomic<bool> g_attr_set[2][2][kMaxDevices];  // [16 rows][steps of 32][device]
 
-auto rows_kernel_of(bool wide) { return wide ? kv8r::rows_kernel<2> : kv8r::rows_kernel<1>; }
+auto rows_kernel_of(bool wide, bool fine) {
+  if (fine) return wide ? kv8r::rows_kernel<2, 2> : kv8r::rows_kernel<1, 2>;
+  return wide ? kv8r::rows_kernel<2, 4> : kv8r::rows_kernel<1, 4>;
+}
 
-int set_rows_attribute(bool wide, int dev) {
-  if (g_attr_set[wide][dev].load(std::memory_order_acquire)) return HSD_OK;
+int set_rows_attribute(bool wide, bool fine, int dev) {
+  if (g_attr_set[wide][fine][dev].load(std::memory_order_acquire)) return HSD_OK;
   int rc = cuda_check(
-      cudaFuncSetAttribute(rows_kernel_of(wide), cudaFuncAttributeMaxDynamicSharedMemorySize,
+      cudaFuncSetAttribute(rows_kernel_of(wide, fine), cudaFuncAttributeMaxDynamicSharedMemorySize,
                            int(kv8r::kSmem)),
       "cudaFuncSetAttribute(rows_kernel)");
   if (rc == HSD_OK)
-    rc = cuda_check(cudaFuncSetAttribute(rows_kernel_of(wide),
+    rc = cuda_check(cudaFuncSetAttribute(rows_kernel_of(wide, fine),
                                          cudaFuncAttributeNonPortableClusterSizeAllowed, 1),
                     "cudaFuncSetAttribute(rows_kernel)");
-  if (rc == HSD_OK) g_attr_set[wide][dev].store(true, std::memory_order_release);
+  if (rc == HSD_OK) g_attr_set[wide][fine][dev].store(true, std::memory_order_release);
   return rc;
 }
 
@@ -838,7 +853,7 @@ struct Device {
 // chip, so this is less than SMs / s.
 int resident_clusters(bool wide, int s, int dev, int sms) {
   if (s == 1) return sms;
-  if (set_rows_attribute(wide, dev) != HSD_OK) return 0;
+  if (set_rows_attribute(wide, false, dev) != HSD_OK) return 0;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(s * sms));
   cfg.blockDim = dim3(kv8r::kThreads);
@@ -850,7 +865,7 @@ int resident_clusters(bool wide, int s, int dev, int sms) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   int n = 0;
-  return cudaOccupancyMaxActiveClusters(&n, rows_kernel_of(wide), &cfg) == cudaSuccess ? n : 0;
+  return cudaOccupancyMaxActiveClusters(&n, rows_kernel_of(wide, false), &cfg) == cudaSuccess ? n : 0;
 }
 
 const Device& current_device() {
@@ -876,33 +891,37 @@ const Device& current_device() {
   return table[dev];
 }
 
-// CTAs per tile and what the launch then takes.  A launch takes about 4.2 us (16 rows
-// a tile: 5.2) and 2.7 us (3.4) for each step of a warp, so the time goes by the waves
-// of clusters and the steps; the join kernel (2 us) lets CTAs be dealt out without
-// regard to clusters, or more than kMaxCluster of them to a tile.  Measured, 12/2
-// heads, one row: 4097 columns 6.7 us with a cluster of 9 (of 8: 9.4), 8193 columns 7.9
-// with 17 CTAs and the join (cluster of 16: 9.6, of 8: 12.0), 16,385 columns 8.1 with 33
-// (cluster of 16: 12.1).
+// CTAs per tile, columns per step, and what the launch then takes.  A launch takes
+// about 4.2 us (16 rows a tile: 5.2) and 2.7 us (3.4) for each step of a warp, 2 us (2.5)
+// if sealed steps have 32 columns instead of 64: those pay where every warp then has
+// one.  So the time goes by the waves of clusters and the steps; the join kernel (2 us)
+// lets CTAs be dealt out without regard to clusters, or more than kMaxCluster of them
+// to a tile.  Measured, 12/2 heads, one row: 1601 columns 5.6 us with steps of 32 (of
+// 64: 6.4), 4097 columns 6.8 with a cluster of 9 and steps of 64 (of 32: 7.6; cluster of
+// 8: 9.4), 8193 columns 7.0 with 33 CTAs, steps of 32 and the join (cluster of 16, steps
+// of 64: 9.6).
 Kv8RowsChoice choose(int q_len, int kv_len, int hq, int hkv) {
   const Device& dev = current_device();
   const int64_t tiles = int64_t(n_tiles(q_len, hq / hkv)) * hkv;
   const bool wide = tile_rows(q_len, hq / hkv) > 8;
-  const int units = (kv_len + 63) / 64;
-  const int most = (units + kv8r::kWarps - 1) / kv8r::kWarps;
-  auto time = [&](int64_t waves, int s) {
-    const int steps = (units + s * kv8r::kWarps - 1) / (s * kv8r::kWarps);
-    return float(waves) * (wide ? 5.2f + 3.4f * float(steps) : 4.2f + 2.7f * float(steps));
-  };
-  Kv8RowsChoice best{1, false, time((tiles + dev.sms - 1) / dev.sms, 1), dev.sms};
-  for (int s = 2; s <= kv8r::kMaxCluster && s <= most; ++s) {
-    const int at_once = dev.clusters[wide][s];
-    if (at_once < 1) continue;
-    const float us = time((tiles + at_once - 1) / at_once, s);
-    if (us < best.us) best = {s, false, us, dev.sms};
+  const float step_us[2][2] = {{2.7f, 2.f}, {3.4f, 2.5f}};  // [16 rows][steps of 32]
+  Kv8RowsChoice best{1, false, false, 3.0e38f, dev.sms};
+  for (int fine = 0; fine < 2; ++fine) {
+    const int units = (kv_len + (fine ? 31 : 63)) / (fine ? 32 : 64);
+    const int most = (units + kv8r::kWarps - 1) / kv8r::kWarps;
+    auto consider = [&](int s, bool join, int64_t waves) {
+      const int steps = (units + s * kv8r::kWarps - 1) / (s * kv8r::kWarps);
+      const float us = float(waves) * ((wide ? 5.2f : 4.2f) + step_us[wide][fine] * float(steps)) +
+                       (join ? 2.f : 0.f);
+      if (us < best.us) best = {s, join, fine != 0, us, dev.sms};
+    };
+    consider(1, false, (tiles + dev.sms - 1) / dev.sms);
+    for (int s = 2; s <= kv8r::kMaxCluster && s <= most; ++s)
+      if (const int at_once = dev.clusters[wide][s])
+        consider(s, false, (tiles + at_once - 1) / at_once);
+    const int64_t s = std::min<int64_t>(dev.sms / tiles, most);
+    if (s > 1) consider(int(s), true, 1);
   }
-  const int64_t s = std::min<int64_t>(dev.sms / tiles, most);
-  if (s > 1 && time(1, int(s)) + 2.f < best.us)
-    best = {int(s), true, time(1, int(s)) + 2.f, dev.sms};
   return best;
 }
 }  // namespace
@@ -945,11 +964,12 @@ int kv8_rows_launch(const Kv8AttnArgs& a, const Kv8RowsChoice& c) {
   CUtensorMap k8, v8, kt, vt;
   const int64_t tail_rows = p.kv_len - p.tail_row0;
   const bool has8 = p.sealed > 0, has_tail = p.sealed < p.kv_len;
+  const int box = c.fine ? 32 : 64;  // rows of a sealed step
   // a side without columns is never loaded; its map describes the other one
   int rc = HSD_OK;
   if (has8) {
-    rc = kv8_map(&k8, a.k8, false, p.sealed, p.hkv, 128, a.k8_head_stride, 64, "k8");
-    if (!rc) rc = kv8_map(&v8, a.v8, false, p.sealed, p.hkv, 128, a.v8_head_stride, 64, "v8");
+    rc = kv8_map(&k8, a.k8, false, p.sealed, p.hkv, 128, a.k8_head_stride, box, "k8");
+    if (!rc) rc = kv8_map(&v8, a.v8, false, p.sealed, p.hkv, 128, a.v8_head_stride, box, "v8");
   }
   if (!rc && has_tail) {
     rc = kv8_map(&kt, a.k_tail, true, tail_rows, p.hkv, a.kt_row_stride, a.kt_head_stride, 32,
@@ -985,9 +1005,9 @@ int kv8_rows_launch(const Kv8AttnArgs& a, const Kv8RowsChoice& c) {
     return HSD_ERR_UNSUPPORTED;
   }
   const bool wide = sp.rows > 8;
-  rc = set_rows_attribute(wide, dev);
+  rc = set_rows_attribute(wide, c.fine, dev);
   if (rc) return rc;
-  rc = launch_pdl(rows_kernel_of(wide),
+  rc = launch_pdl(rows_kernel_of(wide, c.fine),
                   dim3(unsigned(sp.splits), unsigned(p.hkv), unsigned(sp.n_tiles)),
                   dim3(kv8r::kThreads), kv8r::kSmem, a.stream, "rows_kernel launch",
                   c.splits > 1 && !c.join ? unsigned(c.splits) : 0u, k8, v8, kt, vt, p, sp);
