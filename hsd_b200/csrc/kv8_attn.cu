@@ -186,7 +186,9 @@ __global__ void __launch_bounds__(kExpandThreads) expand_kernel(const ExpandPara
     // the absent second half of an odd last block: any finite factors
     const bool pad = t == p.n_kv64 - 1 && (t & 1) == 0;
     if (z == 0) {
-      c->score = (col0 < p.sealed ? p.scale[0][h * p.scale_stride + t] : 1.f) * p.scale_log2;
+      c->score = col0 < p.sealed
+                     ? score_factor(p.scale[0][h * p.scale_stride + t] * p.scale_log2)
+                     : p.scale_log2;
       if (pad) c[1].score = 1.f;
     } else {
       c->log2_v = log2f(v_unit);

@@ -28,6 +28,14 @@ struct Params {
   float scale_log2;
 };
 
+// A factor on sealed columns' scores, never below the smallest normal number: a block of zero keys
+// (scale 2^-100 / 127) times a zero query row's unit (2^-100) is past fp32's range, and
+// 0 times a masked score (-inf) would be NaN.  Scores under such a factor are below
+// 2^-100, as good as 0.  NaN stays.
+__device__ __forceinline__ float score_factor(float x) {
+  return x < 1.1754943508222875e-38f ? 1.1754943508222875e-38f : x;
+}
+
 // Four signed bytes -> two bf16 pairs, exactly.  A byte placed under the bf16
 // exponent of 128 reads 128 + (its low 7 bits); the same with only the sign
 // bit kept reads 128, or 256 when it is set: their difference is the signed

@@ -57,6 +57,7 @@ using kv8a::biased_to_f16;
 using kv8a::bytes_to_f16;
 using kv8a::pack_f16x2;
 using kv8a::Params;
+using kv8a::score_factor;
 
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
@@ -638,7 +639,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t pk[kNB][NT][2];
       float sc[2 * kNB];
 #pragma unroll
-      for (int r = 0; r < 2 * kNB; ++r) sc[r] = a.ks * q_unit[r];
+      for (int r = 0; r < 2 * kNB; ++r) sc[r] = score_factor(a.ks * q_unit[r]);
       if (any) softmax_step<kNB, NT, true>(c, a.bits, masked, sc, a.vs, pg, s, pk);
       if (nxt.col >= 0) load_aside<kNB>(p, nxt, kvh, qt, mrow, a);
       if (!wait_tile(0x802)) break;

@@ -1,0 +1,43 @@
+"""The 8-bit attention where factors vanish: zero query rows, blocks and scales
+of zero, V of unlike size beside blocks of zeros.
+
+Oracle and limits: ``tests/test_gpu_kv8_attention.py``.
+"""
+import pytest
+import torch
+
+from tests import test_gpu_kv8_attention as T
+from tests.test_gpu_kv8_attention_many import many
+
+pytestmark = pytest.mark.gpu
+dev = T.dev
+
+# few rows (8 and 16 a tile) and many
+ROWS = [(1, 4, 2, False), (11, 5, 1, False), (30, 12, 2, False), (900, 12, 2, True)]
+
+
+@pytest.mark.parametrize("q_len,hq,hkv,is_many", ROWS)
+@pytest.mark.parametrize("sm", [None, 1e-20])
+def test_zero_query_rows_over_zero_keys(dev, q_len, hq, hkv, is_many, sm):
+    """A zero query row (unit 2^-100) against a block of zero keys (scale
+    2^-100 / 127) or under a tiny softmax scale: the score factor is below fp32's
+    range, and masked columns still have to vanish."""
+    from hsd_b200.kv8 import Kv8Layer, verify_attention_kv8
+    kv_len, sealed = 500, 448
+    assert many(q_len, kv_len, hq, hkv) == is_many
+    q, data, scale, tail = T.make(dev, hq, hkv, q_len, kv_len, sealed, seed=q_len)
+    q[:, ::2] = 0
+    for b in (1, 2, 5):
+        data[0, :, 64 * b:64 * b + 64] = 0
+        scale[0, :, b] = 2.0 ** -100 / 127
+    g = torch.Generator().manual_seed(1)
+    allowed = (torch.rand(q_len, kv_len, generator=g) < 0.5).to(dev)
+    allowed[0, 64:192] = False            # nothing of two of the blocks
+    allowed[1::3] = False                 # rows that see nothing ...
+    allowed[3::6, 70:75] = True           # ... or a few zero keys alone
+    plan = T.plan_of(allowed)
+    got = verify_attention_kv8(q, Kv8Layer(data[0], data[1], scale[0], scale[1]), sealed, tail[0],
+                               tail[1], plan, scale=sm)
+    torch.cuda.synchronize()
+    plan.raise_on_device_error()
+    T.check(got, T.exact(q, data, scale, tail, sealed, allowed, sm=sm))
