@@ -176,6 +176,9 @@ __global__ void __launch_bounds__(kThreads)
 namespace {
 
 constexpr int kMaxPlanes = 65535;  // grid y
+// Rows beyond any memory: what is below it leaves room for a launch's rows and for
+// bytes (256 a row) in 64 bits.
+constexpr int64_t kMaxRow = int64_t(1) << 48;
 
 int check_kv8(const char* what, const uint64_t* planes, int32_t n_planes, const void* data,
               int64_t plane_stride, const void* scale, int64_t scale_stride, int64_t last_row) {
@@ -203,7 +206,7 @@ extern "C" int hsd_kv8_seal(const uint64_t* src_planes, int32_t n_planes, int64_
                             int32_t block0, int32_t n_blocks, int32_t* status,
                             hsd_stream_t stream) {
   using namespace hsd;
-  if (src_row0 < 0 || block0 < 0 || n_blocks < 0) {
+  if (src_row0 < 0 || src_row0 > kMaxRow || block0 < 0 || n_blocks < 0) {
     hsd_host::set_error("hsd_kv8_seal: bad range (row %lld, blocks %d + %d)",
                         static_cast<long long>(src_row0), block0, n_blocks);
     return HSD_ERR_INVALID_ARG;
@@ -221,7 +224,7 @@ extern "C" int hsd_kv8_unseal(const int8_t* data, int64_t plane_stride, const fl
                               int64_t scale_stride, int32_t n_planes, int64_t row0, int32_t n_rows,
                               const uint64_t* dst_planes, int64_t dst_row0, hsd_stream_t stream) {
   using namespace hsd;
-  if (row0 < 0 || n_rows < 0 || dst_row0 < 0) {
+  if (row0 < 0 || row0 > kMaxRow || n_rows < 0 || dst_row0 < 0 || dst_row0 > kMaxRow) {
     hsd_host::set_error("hsd_kv8_unseal: bad range (rows %lld + %d to %lld)",
                         static_cast<long long>(row0), n_rows, static_cast<long long>(dst_row0));
     return HSD_ERR_INVALID_ARG;

@@ -161,6 +161,12 @@ int32_t i32(const Args& a, int64_t v, const char* name) {
   return static_cast<int32_t>(v);
 }
 
+// Whether rows [row0, row0 + n) lie within `rows` of them (row0, n >= 0: their sum may
+// pass 64 bits).
+bool fits(int64_t row0, int64_t n, int64_t rows) { return n <= rows && row0 <= rows - n; }
+
+constexpr int64_t kMaxRow = int64_t(1) << 48;  // of planes known by address alone
+
 // ---------------------------------------------------------------- rotary
 // (q, k, v, positions, turns, pair_axis, axes, scaling, k_cache, v_cache,
 //  dst_row0, out, num_q_heads, num_kv_heads, status)
@@ -295,7 +301,8 @@ PyObject* kv8_seal(PyObject* const* args, Py_ssize_t n_args) {
   const at::Tensor& data = cache_data(a, 2);
   const at::Tensor& scale = cache_scale(a, 3, data);
   const int64_t src = a.integer(1), row0 = a.integer(4), n = a.integer(5);
-  if (n < 0 || n % 64 || row0 < 0 || row0 % 64 || row0 + n > data.size(3) || src < 0)
+  if (n < 0 || n % 64 || row0 < 0 || row0 % 64 || !fits(row0, n, data.size(3)) || src < 0 ||
+      src > kMaxRow)
     refuse(PyExc_ValueError,
            "seal: %lld rows (a multiple of 64) from row %lld, after %lld of %lld sealed",
            static_cast<long long>(n), static_cast<long long>(src), static_cast<long long>(row0),
@@ -317,9 +324,10 @@ PyObject* kv8_unseal(PyObject* const* args, Py_ssize_t n_args) {
   const at::Tensor& data = cache_data(a, 0);
   const at::Tensor& scale = cache_scale(a, 1, data);
   const int64_t sealed = a.integer(2), row0 = a.integer(4), n = a.integer(5), dst = a.integer(6);
-  if (row0 < 0 || n < 0 || row0 + n > sealed || sealed > data.size(3) || dst < 0)
-    refuse(PyExc_ValueError, "unseal: rows %lld..%lld of %lld to %lld",
-           static_cast<long long>(row0), static_cast<long long>(row0 + n),
+  if (row0 < 0 || n < 0 || !fits(row0, n, sealed) || sealed > data.size(3) || dst < 0 ||
+      dst > kMaxRow)
+    refuse(PyExc_ValueError, "unseal: %lld rows from row %lld of %lld to %lld",
+           static_cast<long long>(n), static_cast<long long>(row0),
            static_cast<long long>(sealed), static_cast<long long>(dst));
   const Planes p = planes_of(a, 3, data, scale);
   const c10::cuda::CUDAGuard guard(p.dev);

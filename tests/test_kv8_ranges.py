@@ -1,0 +1,47 @@
+"""Row ranges of the 8-bit cache and the rotary update that pass 64 bits: refused
+on the host, where their ends would wrap around to small numbers.  No GPU needed."""
+import ctypes as C
+
+import pytest
+import torch
+
+from hsd_b200 import _native as N
+
+A = C.c_void_p(256)
+FAR = 2 ** 63 - 1
+
+
+def test_kv8_ranges_that_wrap_are_refused():
+    lib = N.load()
+
+    def seal(n=1, row0=0, block0=0, blocks=1, stride=64 * 128):
+        return lib.hsd_kv8_seal(A, n, row0, A, stride, A, 1, block0, blocks, None, None)
+
+    def unseal(n=1, row0=0, rows=64, dst=0, stride=64 * 128):
+        return lib.hsd_kv8_unseal(A, stride, A, 1, n, row0, rows, A, dst, None)
+
+    for n in (1, 4):
+        for rc in (seal(n, row0=FAR), seal(n, row0=2 ** 56), unseal(n, row0=FAR),
+                   unseal(n, row0=FAR - 63), unseal(n, row0=2 ** 56), unseal(n, dst=FAR),
+                   unseal(n, dst=2 ** 55)):
+            assert rc == 1, (n, rc, lib.hsd_last_error())
+            assert b"range" in lib.hsd_last_error()
+
+
+def test_kv8_cache_ranges_that_wrap_are_refused():
+    from hsd_b200.kv8 import Kv8Cache
+    c = Kv8Cache(2, 2, 256, device="cpu")
+    planes = torch.zeros(8, dtype=torch.int64)
+    c.sealed = 128
+    for row0, n in ((FAR, 64), (FAR - 10, 64), (64, FAR), (1, FAR)):
+        with pytest.raises(ValueError):
+            c.unseal(planes, row0, n, dst_row0=0)
+    for n in (2 ** 63 - 64, 2 ** 62):
+        with pytest.raises(ValueError):
+            c.seal(planes, n)
+    for row0 in (FAR, 2 ** 56):
+        with pytest.raises(ValueError):
+            c.seal(planes, 64, src_row0=row0)
+        with pytest.raises(ValueError):
+            c.unseal(planes, 0, 64, dst_row0=row0)
+    assert c.sealed == 128
