@@ -186,9 +186,10 @@ PyObject* rope_append_axes(PyObject* const* args, Py_ssize_t n_args) {
   const int64_t n = k.rows;
   if (v.rows != n) refuse(PyExc_ValueError, "%s: k and v row counts differ", a.fn);
   const int64_t row0 = a.integer(10);
-  if (row0 < 0 || row0 + n > kc.rows)
-    refuse(PyExc_ValueError, "%s: rows %lld..%lld past the cache", a.fn,
-           static_cast<long long>(row0), static_cast<long long>(row0 + n));
+  if (row0 < 0 || !fits(row0, n, kc.rows))
+    refuse(PyExc_ValueError, "%s: %lld rows from row %lld on pass the cache's %lld", a.fn,
+           static_cast<long long>(n), static_cast<long long>(row0),
+           static_cast<long long>(kc.rows));
   const int64_t axes = a.integer(6);
   at::Tensor pos = a.tensor(3, "positions");
   if (!pos.is_cuda() || (pos.scalar_type() != at::kLong && pos.scalar_type() != at::kInt))

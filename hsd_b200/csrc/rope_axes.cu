@@ -168,8 +168,9 @@ extern "C" int hsd_rope_append_axes(
   auto a16 = [](const void* x) { return x && (reinterpret_cast<uintptr_t>(x) & 15) == 0; };
   auto a8 = [](const void* x) { return x && (reinterpret_cast<uintptr_t>(x) & 7) == 0; };
   const int64_t qw = int64_t(num_q_heads) * 128, kw = int64_t(num_kv_heads) * 128;
+  // rows beyond any memory would wrap around to others
   if (n_rows < 0 || num_q_heads < 0 || num_kv_heads <= 0 || dst_row0 < 0 ||
-      num_q_heads > 4096 || num_kv_heads > 4096 ||
+      dst_row0 > (int64_t(1) << 48) || num_q_heads > 4096 || num_kv_heads > 4096 ||
       (num_q_heads > 0 && (!a16(q) || !a16(q_out) || q_row_stride < qw || q_out_row_stride < qw)) ||
       !a16(k) || !a16(v) || !a16(k_cache) || !a16(v_cache) || !a8(positions) || !a8(turns) ||
       !pair_axis || k_row_stride < kw || v_row_stride < kw || cache_row_stride < 128 ||

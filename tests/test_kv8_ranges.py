@@ -45,3 +45,27 @@ def test_kv8_cache_ranges_that_wrap_are_refused():
         with pytest.raises(ValueError):
             c.unseal(planes, 0, 64, dst_row0=row0)
     assert c.sealed == 128
+
+
+def test_rope_axes_rows_that_wrap_are_refused():
+    lib = N.load()
+    for row0 in (FAR, 2 ** 56):
+        assert lib.hsd_rope_append_axes(A, 1536, A, 1536, A, 256, A, 256, A, 4, 1, 3, A, A, 1.0, 4, 12,
+                                        2, 128, A, 4096, A, 4096, 128, row0, None, None) == 1
+        assert b"bad arguments" in lib.hsd_last_error()
+
+
+@pytest.mark.gpu
+def test_rope_axes_rows_past_the_cache_are_refused():
+    from hsd_b200.rope import RotaryAxes, rope_append_axes
+    dev = torch.device("cuda:0")
+    rot = RotaryAxes([64], device=dev)
+    x = torch.ones(4, 256, dtype=torch.bfloat16, device=dev)
+    kc = torch.zeros(2, 8, 128, dtype=torch.bfloat16, device=dev)
+    vc = torch.zeros_like(kc)
+    pos = torch.zeros(1, 4, dtype=torch.int64, device=dev)
+    for row0 in (FAR, FAR - 3, 2 ** 62, 5, -1, -FAR):
+        with pytest.raises(ValueError):
+            rope_append_axes(x, x, x, pos, rot, kc, vc, row0)
+    rope_append_axes(None, x, x, pos, rot, kc, vc, 4)
+    assert bool((kc[:, 4:] == 1).all()) and not kc[:, :4].any()
