@@ -161,8 +161,10 @@ __global__ void __launch_bounds__(kExpandThreads) expand_kernel(const ExpandPara
       __syncthreads();
       top = __reduce_max_sync(0xffffffffu, warp_top[lane_id() & (kExpandThreads / 32 - 1)]);
       // v_unit = 2^(e - 6) for a largest value in [2^e, 2^(e + 1)); e as a float's
-      // exponent field, held where both v_unit and its inverse are normal
-      const uint32_t e = top == 0u ? 133u : min(max(top >> 7, 40u), 250u);
+      // exponent field, held where both v_unit and its inverse are normal.  A block of
+      // zeros takes the least, 2^-90, as a sealed one does: the running maximum is that
+      // of score + log2 v_unit, and a larger unit would cost the other columns' P bits.
+      const uint32_t e = min(max(top >> 7, 43u), 250u);
       v_unit = __uint_as_float((e - 6u) << 23);
       const float inv = __uint_as_float((260u - e) << 23);
 #pragma unroll

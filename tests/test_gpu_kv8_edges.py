@@ -41,3 +41,17 @@ def test_zero_query_rows_over_zero_keys(dev, q_len, hq, hkv, is_many, sm):
     torch.cuda.synchronize()
     plan.raise_on_device_error()
     T.check(got, T.exact(q, data, scale, tail, sealed, allowed, sm=sm))
+
+
+@pytest.mark.parametrize("q_len,hq,hkv,is_many", ROWS)
+def test_bf16_block_of_zeros_beside_small_values(dev, q_len, hq, hkv, is_many):
+    """V of 2^-30 with a visible block of zeros among the bf16 columns: the zeros
+    take part in the weights and cost the others none of their bits."""
+    kv_len, sealed = 640, 320
+    q, data, scale, tail = T.make(dev, hq, hkv, q_len, kv_len, sealed, seed=q_len)
+    scale[1] *= 2.0 ** -30
+    tail[1] *= 2.0 ** -30
+    tail[1, :, 384:448] = 0
+    allowed = torch.ones(q_len, kv_len, dtype=torch.bool, device=dev)
+    got = T.run(q, data, scale, tail, sealed, T.plan_of(allowed))
+    T.check(got, T.exact(q, data, scale, tail, sealed, allowed))
