@@ -237,9 +237,13 @@ __device__ __forceinline__ void softmax_step(float (&c)[kNB][NT][4],
           if (!((uint32_t(bits[2 * b + (i & 1)] >> (16 * j)) >> (pg + 8 * (i >> 1))) & 1u))
             c[b][j][i] = -INFINITY;
   }
-  const float shift = kPShift + __log2f(__fdividef(vs, v_unit));
-  // P with the quotient of the V scales; the row sum without it
-  const float unscale = __fdividef(v_unit, vs);
+  // P with the quotient of the V scales; the row sum without it.  Held at 2^-100, where
+  // fp16 P is 0 already (V then adds nothing), so that its inverse and fp32 P stay in
+  // range and the weights count whatever the quotient.
+  const float exact = __fdividef(vs, v_unit);
+  const float quotient = exact < 7.888609052210118e-31f ? 7.888609052210118e-31f : exact;
+  const float shift = kPShift + __log2f(quotient);
+  const float unscale = __fdividef(1.f, quotient);
   const float f = __fdividef(s.unit, v_unit);
   s.unit = v_unit;
   float of[2 * kNB];  // factors on O

@@ -55,3 +55,23 @@ def test_bf16_block_of_zeros_beside_small_values(dev, q_len, hq, hkv, is_many):
     allowed = torch.ones(q_len, kv_len, dtype=torch.bool, device=dev)
     got = T.run(q, data, scale, tail, sealed, T.plan_of(allowed))
     T.check(got, T.exact(q, data, scale, tail, sealed, allowed))
+
+
+@pytest.mark.parametrize("q_len", [1, 3])
+@pytest.mark.parametrize("big", [20, 60, 90])
+def test_sealed_zeros_beside_large_values_few_rows(dev, q_len, big):
+    """Blocks of zeros (scale 2^-100 / 127) beside V of 2^big, several of each to a
+    warp: their quotient is past fp32's range, their weights still count."""
+    hq, hkv, kv_len, sealed = 16, 8, 20000, 19968
+    assert not many(q_len, kv_len, hq, hkv)
+    q, data, scale, tail = T.make(dev, hq, hkv, q_len, kv_len, sealed, seed=q_len)
+    scale[1] *= 2.0 ** big
+    tail[1] = (tail[1].float() * 2.0 ** big).to(torch.bfloat16)
+    g = torch.Generator().manual_seed(big)
+    zero = (torch.rand(sealed // 64, generator=g) < 0.5).to(dev)
+    data[1, :, :sealed][:, zero.repeat_interleave(64)] = 0
+    scale[1, :, :sealed // 64][:, zero] = 2.0 ** -100 / 127
+    allowed = torch.ones(q_len, kv_len, dtype=torch.bool, device=dev)
+    allowed[-1, 64:192] = False
+    T.check(T.run(q, data, scale, tail, sealed, T.plan_of(allowed)),
+            T.exact(q, data, scale, tail, sealed, allowed))
