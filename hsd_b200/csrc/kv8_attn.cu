@@ -100,11 +100,15 @@ __global__ void __launch_bounds__(kExpandThreads) expand_kernel(const ExpandPara
     // A block of next to nothing (zeros are sealed with the scale 2^-100 / 127)
     // takes the scale 2^-90, so that its columns' part of the row sum, formed as
     // P / scale, does not underflow.
-    float tiny = 0.f;
+    bool tiny = false;
+    float of_unit = 1.f;  // what is left of the scale (0: the scale is 0, and so are the values)
     if (z == 1) {
-      const float vs = p.scale[1][h * p.scale_stride + t];
-      v_unit = fmaxf(vs, kMinVScale);
-      if (vs < kMinVScale) tiny = vs / kMinVScale;
+      v_unit = p.scale[1][h * p.scale_stride + t];
+      tiny = v_unit < kMinVScale;
+      if (tiny) {
+        of_unit = v_unit / kMinVScale;
+        v_unit = kMinVScale;
+      }
     }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -116,11 +120,11 @@ __global__ void __launch_bounds__(kExpandThreads) expand_kernel(const ExpandPara
           bytes_to_bf16(in[i], o[2 * i], o[2 * i + 1]);
         } else {
           bytes_to_f16(in[i], o[2 * i], o[2 * i + 1]);
-          if (tiny > 0.f) {
+          if (tiny) {
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
               const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&o[2 * i + k]));
-              o[2 * i + k] = pack_f16x2(x.x * tiny, x.y * tiny);
+              o[2 * i + k] = pack_f16x2(x.x * of_unit, x.y * of_unit);
             }
           }
         }

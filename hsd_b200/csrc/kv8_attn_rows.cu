@@ -224,8 +224,9 @@ __device__ __forceinline__ void softmax_step(float (&c)[kNB][NT][4],
                                              const float (&sc)[2 * kNB], float vs, int pg,
                                              State<kNB>& s, uint32_t (&pk)[kNB][NT][2]) {
   s.unit_max = fmaxf(s.unit_max, vs);
-  const float low = fmaxf(vs, s.unit_max * 8.673617379884035e-19f);
-  const bool keep = vs <= s.unit && vs >= s.unit * 9.5367431640625e-07f;
+  // (2^-110, below what sealing leaves: a unit for scales of 0 alone)
+  const float low = fmaxf(fmaxf(vs, s.unit_max * 8.673617379884035e-19f), 7.703719777548943e-34f);
+  const bool keep = vs > 0.f && vs <= s.unit && vs >= s.unit * 9.5367431640625e-07f;
   const float v_unit = keep ? s.unit : low;
   if (masked) {
 #pragma unroll

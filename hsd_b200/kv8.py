@@ -113,9 +113,10 @@ def verify_attention_kv8(q, layer, sealed, k, v, plan: TilePlan, scale=None, tai
 
     Runs on the device's current stream, with scratch kept per device and
     stream; with many rows it holds the layer's expanded columns (512 bytes
-    per column and KV head).  Scales must be positive, as sealing leaves them.
-    P is rounded to fp16 (few rows: to bf16 over the bf16 columns); scores and
-    sums are fp32.
+    per column and KV head).  Scales must not be negative; 0 stands for a
+    block of zeros.  P is rounded to fp16 (few rows: to bf16 over the bf16
+    columns); scores and sums are fp32.  V's blocks of 64 columns may differ by
+    2^60 in magnitude; beside blocks of zeros V stays below 2^26.
     """
     return N.ops().verify_attention_kv8(q, layer, sealed, k, v, plan.address, plan.status, scale,
                                         tail_row0, out, lse, need_lse)

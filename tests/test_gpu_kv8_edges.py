@@ -75,3 +75,46 @@ def test_sealed_zeros_beside_large_values_few_rows(dev, q_len, big):
     allowed[-1, 64:192] = False
     T.check(T.run(q, data, scale, tail, sealed, T.plan_of(allowed)),
             T.exact(q, data, scale, tail, sealed, allowed))
+
+
+@pytest.mark.parametrize("q_len,hq,hkv,is_many", ROWS)
+@pytest.mark.parametrize("everywhere", [False, True])
+def test_scales_of_zero(dev, q_len, hq, hkv, is_many, everywhere):
+    """Another quantiser's scale of a block of zeros: the block's keys and values
+    are zeros, whatever its bytes."""
+    kv_len, sealed = 500, 448
+    q, data, scale, tail = T.make(dev, hq, hkv, q_len, kv_len, sealed, seed=q_len)
+    g = torch.Generator().manual_seed(2)
+    allowed = (torch.rand(q_len, kv_len, generator=g) < 0.6).to(dev)
+    allowed[0] = False
+    allowed[0, :100] = True
+    if everywhere:
+        scale[:] = 0
+        allowed[:, sealed:] = False
+    else:
+        scale[0, :, [0, 2, 6]] = 0
+        scale[1, :, [0, 1, 5]] = 0
+    got = T.run(q, data, scale, tail, sealed, T.plan_of(allowed))
+    T.check(got, T.exact(q, data, scale, tail, sealed, allowed))
+    if everywhere:
+        assert bool((got[0] == 0).all())
+
+
+@pytest.mark.parametrize("tail_zeros", [False, True])
+def test_zeros_beside_large_values_many_rows(dev, tail_zeros):
+    """Zeros (factor 2^-90) beside V of 2^25 at most, sealed and bf16: their weights
+    still count, down to 2^-24 of a row's largest."""
+    q_len, hq, hkv, kv_len, sealed = 900, 12, 2, 1000, 640
+    assert many(q_len, kv_len, hq, hkv)
+    q, data, scale, tail = T.make(dev, hq, hkv, q_len, kv_len, sealed, seed=1)
+    scale[1] *= 2.0 ** 22
+    tail[1] = (tail[1].float() * 2.0 ** 22).to(torch.bfloat16)
+    for b in (0, 3, 4, 8):
+        data[1, :, 64 * b:64 * b + 64] = 0
+        scale[1, :, b] = 2.0 ** -100 / 127
+    if tail_zeros:
+        tail[1, :, 704:832] = 0
+    allowed = torch.ones(q_len, kv_len, dtype=torch.bool, device=dev)
+    allowed[-1, 64:192] = False
+    T.check(T.run(q, data, scale, tail, sealed, T.plan_of(allowed)),
+            T.exact(q, data, scale, tail, sealed, allowed))
