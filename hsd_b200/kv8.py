@@ -5,8 +5,10 @@ in every step of every layer, and never changes it: compaction moves rows at
 or after the first dropped one, which lie behind the prefix.  So whole
 64-token blocks of the prefix can be *sealed* -- stored as int8 with a scale
 per block, plane (layer, K or V, KV head) -- while the rows behind them, the
-*tail*, stay bf16 and are appended and compacted as before.  64 columns are
-the mask's tile width (BlockMask 128 x 64, D:94-106).
+*tail*, stay bf16 and are appended and compacted as before.  Should a compaction
+reach sealed rows all the same, they have to leave the sealed ones
+(:meth:`Kv8Cache.rows_moved`; ``loop.VerifyLoop(kv8=...)`` does it).  64
+columns are the mask's tile width (BlockMask 128 x 64, D:94-106).
 
 * :meth:`Kv8Cache.seal` / :meth:`Kv8Cache.unseal`: every layer in one launch;
 * :func:`verify_attention_kv8`: the packed verification attention (the
@@ -83,6 +85,15 @@ class Kv8Cache:
         if sealed < 0 or sealed % BLOCK or sealed > self.sealed:
             raise ValueError(f"reset: {sealed} of {self.sealed} sealed rows")
         self.sealed = sealed
+
+    def rows_moved(self, first):
+        """The planes' rows from ``first`` on have been moved or dropped (a
+        compaction; ``counts[1]`` of :func:`hsd_b200.compaction.keep_indices`):
+        keep the blocks in front of it.  Returns the rows still sealed."""
+        if first < 0:
+            raise ValueError(f"rows_moved: row {first}")
+        self.sealed = min(self.sealed, first // BLOCK * BLOCK)
+        return self.sealed
 
     def layer(self, l) -> Kv8Layer:
         """Layer ``l``'s tensors (views), for :func:`verify_attention_kv8`."""

@@ -62,7 +62,10 @@ class VerifyLoop:
     compacted alongside the mask; pass
     ``kv_planes`` (device int64 plane addresses, see
     :func:`hsd_b200.compaction.plane_pointers`) and ``row_bytes`` to have
-    model caches compacted in place too.
+    model caches compacted in place too.  ``kv8``: a
+    :class:`hsd_b200.kv8.Kv8Cache` sealed from those planes' rows; blocks that
+    a compaction moves rows of leave it (``kv8.sealed`` shrinks, and their
+    columns are bf16 again until they are sealed anew).
     """
 
     def __init__(self, prompts, drafts, *, eos_token_id, max_new_tokens, pad_token_id=0,
@@ -73,7 +76,7 @@ class VerifyLoop:
                  kv_capacity=None, spec_thresh=1.0, tree_thresh=1.0, variant="dots",
                  formula_tokens=(3, 1099), spec_mode="fmst", spec_topk=3, spec_margin=2.0,
                  packed=None, page_block=False, pad_rows_inherit=False, compact_hook=None,
-                 track_kv_tokens=True, device="cuda"):
+                 track_kv_tokens=True, kv8=None, device="cuda"):
         if packed is not None:
             # the caller's packed prefill: (input_ids, position_ids, pointer)
             p_ids, p_pos, p_ptr = packed[:3]
@@ -114,6 +117,10 @@ class VerifyLoop:
         self.ratio = (self.spec_thresh < 1.0 or self.tree_thresh < 1.0
                       or (variant == "hunyuan" and self.tree_decode))
         self.kv_planes, self.row_bytes = kv_planes, int(row_bytes)
+        if kv8 is not None and (kv_planes is None or self.row_bytes != 256
+                                or kv_planes.numel() != 2 * kv8.layers * kv8.num_kv_heads):
+            raise ValueError("kv8 needs the planes it is sealed from (kv_planes, row_bytes=256)")
+        self.kv8 = kv8
         self.drafts = [list(map(int, d)) for d in drafts]
         lens = [len(p) for p in prompts]
         if kv_capacity is None:
@@ -417,7 +424,7 @@ class VerifyLoop:
         o += nb * len(R)
         code = int(h[o])
         o += 1
-        n_keep = int(h[o])
+        n_keep, first_moved = int(h[o]), int(h[o + 1])
         o += 2
         blk = h[o:o + nb * 16].reshape(nb, 16).copy()
         o += nb * 16
@@ -490,6 +497,8 @@ class VerifyLoop:
             if self.kv_planes is not None:
                 compact_kv(self.kv_planes, self.row_bytes, keep_idx, counts=counts,
                            status=self.status)
+            if self.kv8 is not None:
+                self.kv8.rows_moved(first_moved)
             if self.compact_hook is not None:
                 self.compact_hook(keep_idx, counts, n_keep)
             if self.kv_tokens is not None:
