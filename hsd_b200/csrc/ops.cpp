@@ -366,20 +366,24 @@ Heads heads_of(const Args& a, const at::Tensor& t, const char* name) {
   return h;
 }
 
-// Scratch of (device, current stream), grown to fit.  A call that is being captured
-// into a graph gets scratch of its own from the graph's pool, so graphs that share
-// no stream share no scratch either (replays of one graph never overlap).
+// Scratch of a call.  Up to kKeptScratch (few rows: partial rows for one CTA per SM)
+// it is kept per device and current stream.  More (many rows: a layer's expanded
+// columns, 512 bytes per column and KV head) comes from the caching allocator and goes
+// back to it with the call, so that it serves other tensors between calls and no stream
+// holds the largest size ever seen; the next call on the stream runs after this one.  So
+// does a call that is being captured into a graph, from the graph's pool: graphs that
+// share no stream share no scratch either (replays of one graph never overlap).
+constexpr int64_t kKeptScratch = 2 << 20;
+
 at::Tensor workspace(int64_t need, const c10::Device& dev) {
-  const auto opt = at::TensorOptions().dtype(at::kByte).device(dev);
-  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
-    return at::empty({need + 256}, opt);
+  if (need > kKeptScratch ||
+      c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
+    return at::detail::empty_cuda({need + 256}, at::kByte, dev, std::nullopt);
   // never destroyed: tensors must not outlive the allocator at exit
   static auto* cached = new std::map<std::pair<int, void*>, at::Tensor>;
   at::Tensor& t = (*cached)[{dev.index(), c10::cuda::getCurrentCUDAStream(dev.index()).stream()}];
-  if (!t.defined() || t.numel() < need + 256) {
-    t = at::Tensor();
-    t = at::empty({std::max<int64_t>(need, 1 << 20) + 256}, opt);
-  }
+  if (!t.defined())
+    t = at::detail::empty_cuda({kKeptScratch + 256}, at::kByte, dev, std::nullopt);
   return t;
 }
 

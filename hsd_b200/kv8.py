@@ -122,9 +122,9 @@ def verify_attention_kv8(q, layer, sealed, k, v, plan: TilePlan, scale=None, tai
     Returns ``(out [Q, Hq, 128] bf16, lse [Hq, Q] fp32 natural log or None)``;
     rows that see nothing give 0 and -inf.
 
-    Runs on the device's current stream, with scratch kept per device and
-    stream; with many rows it holds the layer's expanded columns (512 bytes
-    per column and KV head).  Scales must not be negative; 0 stands for a
+    Runs on the device's current stream, with 2 MB of scratch kept per device
+    and stream; with many rows the layer's expanded columns (512 bytes per
+    column and KV head) are held for the call, from PyTorch's allocator.  Scales must not be negative; 0 stands for a
     block of zeros.  P is rounded to fp16 (few rows: to bf16 over the bf16
     columns); scores and sums are fp32.  V's blocks of 64 columns may differ by
     2^60 in magnitude; beside blocks of zeros V stays below 2^26.
