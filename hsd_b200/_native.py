@@ -115,6 +115,7 @@ SIGNATURES = [
     ("hsd_kv8_seal", C.c_int, [_P, _I32, _I64, _P, _I64, _P, _I64, _I32, _I32, _P, _P]),
     ("hsd_kv8_unseal", C.c_int, [_P, _I64, _P, _I64, _I32, _I64, _I32, _P, _I64, _P]),
     ("hsd_kv8_attention_workspace_bytes", _SZ, [_I32, _I32, _I32, _I32]),
+    ("hsd_kv8_attention_choice", C.c_int, [_I32, _I32, _I32, _I32, _P]),
     ("hsd_verify_attention_kv8", C.c_int,
      [_P, _I64, _I64, _P, _I64, _P, _I64, _P, _P, _I64, _I32, _P, _I64, _I64, _P, _I64, _I64,
       _I32, _P, _P, _I32, _I32, _I32, _I32, _I32, _F, C.POINTER(Plan), _P, _SZ, _P, _P]),

@@ -335,6 +335,22 @@ extern "C" size_t hsd_kv8_attention_workspace_bytes(int32_t q_len, int32_t kv_le
   return choose_path(q_len, kv_len, num_q_heads, num_kv_heads).bytes;
 }
 
+extern "C" int hsd_kv8_attention_choice(int32_t q_len, int32_t kv_len, int32_t num_q_heads,
+                                        int32_t num_kv_heads, int32_t choice[4]) {
+  if (q_len <= 0 || kv_len <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 ||
+      num_q_heads % num_kv_heads || !choice) {
+    hsd_host::set_error("hsd_kv8_attention_choice: bad arguments (q_len=%d kv_len=%d heads=%d/%d)",
+                        q_len, kv_len, num_q_heads, num_kv_heads);
+    return HSD_ERR_INVALID_ARG;
+  }
+  const Path path = choose_path(q_len, kv_len, num_q_heads, num_kv_heads);
+  choice[0] = path.many;
+  choice[1] = path.many ? 0 : path.rows.splits;
+  choice[2] = path.many ? 0 : path.rows.join;
+  choice[3] = path.many ? 0 : (path.rows.fine ? 32 : 64);
+  return HSD_OK;
+}
+
 extern "C" int hsd_verify_attention_kv8(
     const void* q, int64_t q_row_stride, int64_t q_head_stride, const int8_t* k8,
     int64_t k8_head_stride, const int8_t* v8, int64_t v8_head_stride, const float* k_scale,

@@ -407,6 +407,12 @@ int hsd_kv8_unseal(const int8_t *data, int64_t plane_stride, const float *scale,
  * contents; calls sharing one must not overlap in time. */
 size_t hsd_kv8_attention_workspace_bytes(int32_t q_len, int32_t kv_len, int32_t num_q_heads,
                                          int32_t num_kv_heads);
+/* What hsd_verify_attention_kv8 launches for these sizes on the current device, for
+ * tests and diagnostics: choice[0] 1: the columns expanded first (many rows), then
+ * 0 in the others; 0: few rows, choice[1] CTAs to a tile, choice[2] 1: joined by a
+ * second launch, 0: as a cluster, choice[3] sealed columns of a step (32 or 64). */
+int hsd_kv8_attention_choice(int32_t q_len, int32_t kv_len, int32_t num_q_heads,
+                             int32_t num_kv_heads, int32_t choice[4]);
 int hsd_verify_attention_kv8(const void *q, int64_t q_row_stride, int64_t q_head_stride,
                              const int8_t *k8, int64_t k8_head_stride, const int8_t *v8,
                              int64_t v8_head_stride, const float *k_scale, const float *v_scale,
