@@ -11,10 +11,12 @@
 //
 // Angles.  A position of 10^5 times a frequency loses 0.004 rad in fp32, so
 // the frequency is kept as turns per position in 64-bit fixed point (units of
-// 2^-64 turn): position * turns modulo 2^64 is the fraction of a turn, exact
-// for any int64 position, negative ones included (two's complement wraps as
-// turns do).  The upper 32 bits, as a signed fraction of a half turn, feed
-// sincospif.  Error: 2^-25 half turns, that of rounding the angle to fp32.
+// 2^-64 turn): position * turns modulo 2^64 is the fraction of a turn, a product
+// without error for any int64 position, negative ones included (two's complement
+// wraps as turns do).  The upper 32 bits, as a signed fraction of a half turn, feed
+// sincospif.  Error in half turns: 2^-25 for rounding the angle to fp32, 2^-31 for
+// the bits below, and |position| * 2^-64 for the frequency's rounding to 2^-64 turn,
+// which is below the first up to positions of 2^39 (at 2^63 nothing is left).
 //
 // Work: a CTA takes a few rows; 64 threads per row compute the row's cosines
 // and sines once into shared memory, and all heads use them.  The rows' first

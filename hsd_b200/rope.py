@@ -145,11 +145,12 @@ def rope_append_axes(q, k, v, positions, rotary, k_cache, v_cache, dst_row0, out
 
     q, k, v, k_cache, v_cache, dst_row0 as in :func:`rope_append` (k and v may
     have different row strides); positions: int64 ``[A, Q]`` (``[1, A, Q]`` and
-    ``[A, 1, Q]`` too; any strides, an expanded row included), any values;
+    ``[A, 1, Q]`` too; any strides, an expanded row included);
     rotary: the :class:`RotaryAxes` of the model.  The queries are rotated in
     place, or into ``out`` (``[..., Q, Hq * 128]`` bf16, not overlapping q).
-    Arithmetic is fp32 with one rounding to bf16, with angles exact to fp32 at
-    any position (:func:`rope_append` reproduces torch's bf16 products).
+    Arithmetic is fp32 with one rounding to bf16 (:func:`rope_append` reproduces
+    torch's bf16 products); angles are off by 2^-25 half turns, that of fp32, up to
+    positions of 2^39, and by ``|position| * 2**-64`` half turns beyond.
     Returns the rotated queries as a ``[1, Hq, Q, 128]`` view, or None when q
     is None.  Asynchronous on the device's current stream.
     """
