@@ -153,6 +153,10 @@ def rope_append_axes(q, k, v, positions, rotary, k_cache, v_cache, dst_row0, out
     positions of 2^39, and by ``|position| * 2**-64`` half turns beyond.
     Returns the rotated queries as a ``[1, Hq, Q, 128]`` view, or None when q
     is None.  Asynchronous on the device's current stream.
+
+    A model that normalises queries and keys per head after the rotation (the
+    HunYuan decoder) does so on the returned view and, in place, on the rows
+    written to ``k_cache``; nothing is normalised here.
     """
     return N.ops().rope_append_axes(q, k, v, positions, rotary.turns, rotary.pair_axis,
                                     rotary.axes, rotary.scaling, k_cache, v_cache, dst_row0, out,
