@@ -158,6 +158,14 @@ def load():
 _ops = None
 
 
+def ops_target():
+    """What the Python binding is built for: its C++ classes and its C API are
+    those of one PyTorch and one interpreter."""
+    import sys
+    import torch
+    return f"torch {torch.__version__}, {sys.implementation.cache_tag}"
+
+
 def ops():
     """The compiled Python binding ``_ops.so`` (csrc/ops.cpp), loaded once."""
     global _ops
@@ -173,6 +181,9 @@ def ops():
             spec.loader.exec_module(module)
         except ImportError as e:
             raise HSDNativeError(f"cannot load {path}: {e}") from e
+        if module.built_for != ops_target():
+            raise HSDNativeError(f"{path} was built for {module.built_for}, this is "
+                                 f"{ops_target()}: rebuild it with `python -m hsd_b200.build`")
         _ops = module
     return _ops
 

@@ -9,7 +9,8 @@ library loads next to PyTorch's own runtime without version coupling.  Then
 compiles ``csrc/ops.cpp``, the Python binding of the entry points whose calls
 have to be cheap on the host (``hsd_b200/_ops.so``; it links PyTorch and the
 library).  The build is incremental: nothing is recompiled when the outputs
-are newer than every source and header.
+are newer than every source and header, and the binding was built for the
+PyTorch and the interpreter that run this.
 """
 from __future__ import annotations
 
@@ -20,12 +21,15 @@ import subprocess
 import sys
 import sysconfig
 
+from ._native import ops_target
+
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 LIB = os.path.join(PKG, "libhsd_b200.so")
 OPS = os.path.join(PKG, "_ops.so")
+OPS_STAMP = os.path.join(PKG, "_build", "ops_built_for.txt")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -53,7 +57,16 @@ def _newer(out, deps):
 
 
 def up_to_date():
-    return _newer(LIB, _deps()) and _newer(OPS, _ops_deps())
+    return _newer(LIB, _deps()) and _ops_up_to_date()
+
+
+def _ops_up_to_date():
+    """The binding is newer than its sources and built for this PyTorch and
+    interpreter (a stamp beside the object files says for which)."""
+    if not _newer(OPS, _ops_deps()) or not os.path.exists(OPS_STAMP):
+        return False
+    with open(OPS_STAMP) as f:
+        return f.read() == ops_target()
 
 
 def _ops_deps():
@@ -75,6 +88,7 @@ def _ops_command(out):
     lib = os.path.join(home, "lib")
     return [cxx, "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            f'-DHSD_BUILT_FOR="{ops_target()}"',
             os.path.join(CSRC, "ops.cpp"), "-o", out] + ["-I" + d for d in inc] + \
         ["-L" + PKG, "-l:libhsd_b200.so", "-Wl,-rpath,$ORIGIN", "-L" + lib, "-ltorch_python",
          "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_cuda"]
@@ -83,7 +97,7 @@ def _ops_command(out):
 def build(verbose=False, force=False, jobs=None):
     if force or not _newer(LIB, _deps()):
         _build_library(verbose)
-    if force or not _newer(OPS, _ops_deps()):
+    if force or not _ops_up_to_date():
         tmp = OPS + ".tmp"
         r = subprocess.run(_ops_command(tmp), stdout=subprocess.PIPE, stderr=subprocess.STDOUT,
                            text=True)
@@ -92,6 +106,9 @@ def build(verbose=False, force=False, jobs=None):
         if r.returncode:
             raise RuntimeError("the Python binding (csrc/ops.cpp) failed to build")
         os.replace(tmp, OPS)
+        os.makedirs(os.path.dirname(OPS_STAMP), exist_ok=True)
+        with open(OPS_STAMP, "w") as f:
+            f.write(ops_target())
     return LIB
 
 

@@ -532,4 +532,11 @@ PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "hsd_b200._ops", nullptr, -1, kMet
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__ops(void) { return PyModule_Create(&kModule); }
+PyMODINIT_FUNC PyInit__ops(void) {
+  PyObject* m = PyModule_Create(&kModule);
+  if (m && PyModule_AddStringConstant(m, "built_for", HSD_BUILT_FOR)) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}
