@@ -44,8 +44,10 @@ class Kv8Cache:
     ``data``: int8 ``[layers, 2, Hkv, capacity, 128]``, ``scale``: fp32
     ``[layers, 2, Hkv, capacity // 64]``; the plane order is that of
     ``plane_pointers`` over the layers' K and V caches in turn.  ``sealed``
-    rows (a multiple of 64) are in use.  Calls run on the device's current
-    stream; ``status`` (int32, one word per cache) collects device reports.
+    rows (a multiple of 64) are in use, counted on the host when a call is made
+    (or captured: a graph's replays seal the rows of the capture).  Calls run on
+    the device's current stream; ``status`` (int32, one word per cache) collects
+    device reports.
     """
 
     def __init__(self, layers, num_kv_heads, capacity, device="cuda"):
@@ -101,8 +103,11 @@ class Kv8Cache:
         return Kv8Layer(d[0], d[1], s[0], s[1])
 
     def raise_on_device_error(self):
+        """Raise, and clear the report, if a call since the last one sealed an
+        infinity or NaN."""
         code = int(self.status.item())
         if code:
+            self.status.zero_()
             raise N.HSDError(f"device status 0x{code:x} while sealing (0x{N.HSD_DEV_BAD_VALUE:x}: "
                              "an infinity or NaN among the rows)")
 
