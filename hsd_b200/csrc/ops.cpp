@@ -129,6 +129,9 @@ Cache cache_of(const Args& a, const at::Tensor& t, const char* name) {
   c.rows = t.size(-2);
   c.row_stride = c.rows > 1 ? t.stride(-2) : 128;
   c.head_stride = c.heads > 1 ? t.stride(-3) : 128;
+  // rows are written: heads or rows in one place (an expanded tensor) would be a race
+  if (c.heads > 1 && c.rows > 0 && c.head_stride == 0)
+    refuse(PyExc_ValueError, "%s: %s has its heads in one place (stride 0)", a.fn, name);
   return c;
 }
 

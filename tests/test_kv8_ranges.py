@@ -69,3 +69,21 @@ def test_rope_axes_rows_past_the_cache_are_refused():
             rope_append_axes(x, x, x, pos, rot, kc, vc, row0)
     rope_append_axes(None, x, x, pos, rot, kc, vc, 4)
     assert bool((kc[:, 4:] == 1).all()) and not kc[:, :4].any()
+
+
+@pytest.mark.gpu
+def test_rope_axes_caches_with_heads_in_one_place_are_refused():
+    """Expanded caches: every head would be written to the same rows."""
+    from hsd_b200.rope import RotaryAxes, rope_append_axes
+    dev = torch.device("cuda:0")
+    rot = RotaryAxes([64], device=dev)
+    x = torch.ones(4, 256, dtype=torch.bfloat16, device=dev)
+    kc = torch.zeros(2, 8, 128, dtype=torch.bfloat16, device=dev)
+    pos = torch.zeros(1, 4, dtype=torch.int64, device=dev)
+    one_head = torch.zeros(1, 8, 128, dtype=torch.bfloat16, device=dev).expand(2, 8, 128)
+    one_row = torch.zeros(2, 1, 128, dtype=torch.bfloat16, device=dev).expand(2, 8, 128)
+    for k_cache, v_cache in ((one_head, kc), (kc, one_head), (one_row, one_row)):
+        with pytest.raises((ValueError, N.HSDError)):
+            rope_append_axes(None, x, x, pos, rot, k_cache, v_cache, 0)
+    torch.cuda.synchronize()
+    assert not kc.any() and not one_head.any() and not one_row.any()
