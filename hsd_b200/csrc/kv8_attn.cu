@@ -14,7 +14,8 @@
 // 2 heads it is latency (7.1 us alone from cold caches, about 3.5 in a stream of steps,
 // where the attention's setup runs under it).  Both together: 51.7 us for 2176 rows,
 // 12/2 heads, 4800 columns (the bf16 kernel alone 47.8), 215 us for 2049 rows and
-// 18,450 columns (210).
+// 18,450 columns (210) at 1965 MHz; a long stream of the latter runs into the board's
+// 1000 W limit, at 1785 MHz, and takes 239 a call.
 #include "kv8_attn.cuh"
 #include "verify_attn.cuh"
 
@@ -228,7 +229,8 @@ ManyLayout many_layout(int32_t kv_len, int32_t hkv) {
   return m;
 }
 
-// Rows kernel or many rows, by the time each takes.  Many rows: 22 us, the expansion
+// Rows kernel or many rows, by the time each takes over the whole cache (what the plan
+// leaves visible of it is known on the device alone).  Many rows: 22 us, the expansion
 // (1.3e-4 us a column and KV head), 2.05 us per SM for every 128 rows x 128 columns x
 // two heads, and 1.2 us for each part of an item (128 rows, two heads) that its first
 // CTA merges when all SMs share few items.  Measured (rows / many, us): 12/2 heads, 1600

@@ -397,9 +397,9 @@ int hsd_kv8_unseal(const int8_t *data, int64_t plane_stride, const float *scale,
  * and -inf, and what stands in a bf16 column that no query row sees does not
  * matter.  Scales must not be negative (0: a block of zeros).  V's blocks of
  * 64 columns may differ by 2^60 in magnitude (beside blocks of zeros: V below
- * 2^26, where the zeros' weights still count).  P is rounded to fp16 (few rows: to bf16
- * over the bf16 columns); scores, sums and joined rows are fp32, the partial
- * rows of items cut between SMs fp16 times a power of two per row.
+ * 2^26, where the zeros' weights still count).  P is rounded to fp16 (few rows:
+ * to bf16 over the bf16 columns); scores, sums and joined rows are fp32, the
+ * partial rows of items cut between SMs fp16 times a power of two per row.
  * Two paths by size: few rows read the cache as it is; many first expand the
  * layer's columns into the workspace, which then holds 512 bytes per column
  * and KV head.

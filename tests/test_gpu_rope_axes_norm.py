@@ -42,7 +42,7 @@ def test_norm_between_rotation_and_attention():
     rot = OA.rotate(qkv[:, :b].double().numpy().reshape(n, hq + hkv, 128), pos[0].numpy(),
                     OA.pair_axis(sections), freq)
     rms = np.sqrt((rot ** 2).mean(-1, keepdims=True) + 1e-5)
-    rot = rot / rms * np.concatenate([np.repeat(w[:1], hq, 0), np.repeat(w[1:], hkv, 0)])[None]
+    rot = rot / rms * np.concatenate([np.repeat(w[:1].numpy(), hq, 0), np.repeat(w[1:].numpy(), hkv, 0)])[None]
     got = np.concatenate([q[0].transpose(0, 1).double().cpu().numpy(),
                           kc[:, at:at + n].transpose(0, 1).double().cpu().numpy()], 1)
     assert (np.abs(got - rot) <= 2.0 ** -7 * np.abs(rot).max(-1, keepdims=True)).all()
