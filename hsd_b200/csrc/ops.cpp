@@ -509,6 +509,23 @@ PyObject* verify_attention_kv8(PyObject* const* args, Py_ssize_t n_args) {
   return r;
 }
 
+// torch.OutOfMemoryError, which programs catch to free memory and call again.
+PyObject* out_of_memory() {
+  static PyObject* cls = nullptr;
+  if (!cls) {
+    PyObject* m = PyImport_ImportModule("torch");
+    if (m) {
+      cls = PyObject_GetAttrString(m, "OutOfMemoryError");
+      Py_DECREF(m);
+    }
+    if (!cls) {
+      PyErr_Clear();
+      return PyExc_RuntimeError;
+    }
+  }
+  return cls;
+}
+
 template <PyObject* (*F)(PyObject* const*, Py_ssize_t)>
 PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
   try {
@@ -516,6 +533,8 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
   } catch (const Refused& r) {
     PyErr_SetString(r.type, r.what.c_str());
   } catch (const PythonError&) {
+  } catch (const c10::OutOfMemoryError& e) {
+    PyErr_SetString(out_of_memory(), e.what_without_backtrace());
   } catch (const c10::Error& e) {
     PyErr_SetString(PyExc_RuntimeError, e.what_without_backtrace());
   } catch (const std::exception& e) {

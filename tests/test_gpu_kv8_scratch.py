@@ -52,3 +52,33 @@ def test_few_rows_fit_the_kept_scratch(dev):
             for kv_len in (65, 1000, 8193, 40000, 131072, 1 << 20):
                 need = lib.hsd_kv8_attention_workspace_bytes(q_len, kv_len, hq, hkv)
                 assert need <= 2 << 20 or need >= 512 * hkv * kv_len
+
+
+def test_out_of_memory_is_pytorchs_error(dev):
+    """With PyTorch's own limit set (nothing is allocated beyond it), a call that
+    cannot have its scratch raises torch.OutOfMemoryError, and runs once it can."""
+    hq, hkv, q_len, kv_len, sealed = 8, 8, 700, 20000, 19968
+    assert many(q_len, kv_len, hq, hkv)
+    allowed = torch.ones(q_len, kv_len, dtype=torch.bool, device=dev)
+    x = T.make(dev, hq, hkv, q_len, kv_len, sealed, seed=3)
+    plan = T.plan_of(allowed)
+    want = T.run(*x, sealed, plan)
+    torch.cuda.synchronize()
+    del allowed
+    torch.cuda.empty_cache()
+    total = torch.cuda.get_device_properties(dev).total_memory
+    try:
+        torch.cuda.set_per_process_memory_fraction(
+            (torch.cuda.memory_reserved(dev) + (24 << 20)) / total, dev)
+        held = []                         # what the allocator still has free
+        for size in (32 << 20, 4 << 20):
+            with pytest.raises(torch.OutOfMemoryError):
+                for _ in range(1000):
+                    held.append(torch.empty(size, dtype=torch.uint8, device=dev))
+        with pytest.raises(torch.OutOfMemoryError):
+            T.run(*x, sealed, plan)
+        del held
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0, dev)
+    got = T.run(*x, sealed, plan)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
