@@ -44,7 +44,13 @@ struct ExpandParams {
 };
 
 constexpr int kExpandThreads = 256;
-constexpr float kMinVScale = 8.077935669463161e-28f;  // 2^-90
+// Least V factor, 2^-60: what blocks of zeros take, and where smaller V keeps its bits
+// in fp16 down to 2^-73.  The running maximum is that of score + log2 of the factor, so
+// a factor far below the others' would lose its columns' part of the row sum in the
+// exponentials that bring sums to a common maximum (below 2^-126 they are 0): beside V
+// of 2^b, weights below 2^-(72 - b) of the largest are lost.
+constexpr float kMinVScale = 8.673617379884035e-19f;
+constexpr uint32_t kMinVExponent = 127 - 60 + 6;
 
 // Columns of a 64-column tile that some query row sees: a warp per query tile, four
 // tiles' loads in flight.
@@ -99,7 +105,7 @@ __global__ void __launch_bounds__(kExpandThreads) expand_kernel(const ExpandPara
     v[0] = __ldcs(src + tid);
     v[1] = __ldcs(src + tid + kExpandThreads);
     // A block of next to nothing (zeros are sealed with the scale 2^-100 / 127)
-    // takes the scale 2^-90, so that its columns' part of the row sum, formed as
+    // takes the least factor, so that its columns' part of the row sum, formed as
     // P / scale, does not underflow.
     bool tiny = false;
     float of_unit = 1.f;  // what is left of the scale (0: the scale is 0, and so are the values)
@@ -167,9 +173,9 @@ __global__ void __launch_bounds__(kExpandThreads) expand_kernel(const ExpandPara
       top = __reduce_max_sync(0xffffffffu, warp_top[lane_id() & (kExpandThreads / 32 - 1)]);
       // v_unit = 2^(e - 6) for a largest value in [2^e, 2^(e + 1)); e as a float's
       // exponent field, held where both v_unit and its inverse are normal.  A block of
-      // zeros takes the least, 2^-90, as a sealed one does: the running maximum is that
-      // of score + log2 v_unit, and a larger unit would cost the other columns' P bits.
-      const uint32_t e = min(max(top >> 7, 43u), 250u);
+      // zeros takes the least, as a sealed one does: the running maximum is that of
+      // score + log2 v_unit, and a larger unit would cost the other columns' P bits.
+      const uint32_t e = min(max(top >> 7, kMinVExponent), 250u);
       v_unit = __uint_as_float((e - 6u) << 23);
       const float inv = __uint_as_float((260u - e) << 23);
 #pragma unroll

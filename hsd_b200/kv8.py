@@ -132,7 +132,7 @@ def verify_attention_kv8(q, layer, sealed, k, v, plan: TilePlan, scale=None, tai
     column and KV head) are held for the call, from PyTorch's allocator.  Scales must not be negative; 0 stands for a
     block of zeros.  P is rounded to fp16 (few rows: to bf16 over the bf16
     columns); scores and sums are fp32.  V's blocks of 64 columns may differ by
-    2^60 in magnitude; beside blocks of zeros V stays below 2^26.
+    2^60 in magnitude, from 2^-73 to 2^80 (beside blocks of zeros: to 2^48).
     """
     return N.ops().verify_attention_kv8(q, layer, sealed, k, v, plan.address, plan.status, scale,
                                         tail_row0, out, lse, need_lse)

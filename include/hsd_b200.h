@@ -396,8 +396,8 @@ int hsd_kv8_unseal(const int8_t *data, int64_t plane_stride, const float *scale,
  * and the tails are those of hsd_verify_attention; fully masked rows give 0
  * and -inf, and what stands in a bf16 column that no query row sees does not
  * matter.  Scales must not be negative (0: a block of zeros).  V's blocks of
- * 64 columns may differ by 2^60 in magnitude (beside blocks of zeros: V below
- * 2^26, where the zeros' weights still count).  P is rounded to fp16 (few rows:
+ * 64 columns may differ by 2^60 in magnitude, from 2^-73 to 2^80 (beside blocks
+ * of zeros: to 2^48, where the zeros' weights still count).  P is rounded to fp16 (few rows:
  * to bf16 over the bf16 columns); scores, sums and joined rows are fp32, the
  * partial rows of items cut between SMs fp16 times a power of two per row.
  * Two paths by size: few rows read the cache as it is; many first expand the

@@ -102,8 +102,8 @@ def test_scales_of_zero(dev, q_len, hq, hkv, is_many, everywhere):
 
 @pytest.mark.parametrize("tail_zeros", [False, True])
 def test_zeros_beside_large_values_many_rows(dev, tail_zeros):
-    """Zeros (factor 2^-90) beside V of 2^25 at most, sealed and bf16: their weights
-    still count, down to 2^-24 of a row's largest."""
+    """Zeros beside V of 2^25 at most, sealed and bf16: their weights still count,
+    down to 2^-24 of a row's largest."""
     q_len, hq, hkv, kv_len, sealed = 900, 12, 2, 1000, 640
     assert many(q_len, kv_len, hq, hkv)
     q, data, scale, tail = T.make(dev, hq, hkv, q_len, kv_len, sealed, seed=1)
@@ -116,5 +116,40 @@ def test_zeros_beside_large_values_many_rows(dev, tail_zeros):
         tail[1, :, 704:832] = 0
     allowed = torch.ones(q_len, kv_len, dtype=torch.bool, device=dev)
     allowed[-1, 64:192] = False
+    T.check(T.run(q, data, scale, tail, sealed, T.plan_of(allowed)),
+            T.exact(q, data, scale, tail, sealed, allowed))
+
+
+@pytest.mark.parametrize("q_len,hq,hkv", [(634, 7, 1), (900, 12, 2)])
+@pytest.mark.parametrize("big", [14, 40])
+def test_zeros_keep_their_weights_when_items_are_joined(dev, q_len, hq, hkv, big):
+    """A sealed prefix of zeros (scores of 0) and bf16 columns with V of 2^big and
+    scores up to 20: the prefix's share of the sum, e^-15 a column, outlives the
+    join of an item's parts, some of which hold nothing but zeros."""
+    from hsd_b200.kv8 import Kv8Layer, verify_attention_kv8
+    kv_len, sealed = 9013, 2496
+    assert many(q_len, kv_len, hq, hkv)
+    q, data, scale, tail = T.make(dev, hq, hkv, q_len, kv_len, sealed, seed=big)
+    data[:] = 0
+    scale[:] = 2.0 ** -100 / 127
+    tail[1] = (tail[1].float() * 2.0 ** big).to(torch.bfloat16)
+    allowed = torch.ones(q_len, kv_len, dtype=torch.bool, device=dev)
+    plan = T.plan_of(allowed)
+    got = verify_attention_kv8(q, Kv8Layer(data[0], data[1], scale[0], scale[1]), sealed, tail[0],
+                               tail[1], plan, scale=0.3)
+    torch.cuda.synchronize()
+    plan.raise_on_device_error()
+    T.check(got, T.exact(q, data, scale, tail, sealed, allowed, sm=0.3))
+
+
+@pytest.mark.parametrize("small", [-40, -60])
+def test_small_values_many_rows(dev, small):
+    """V of 2^small throughout, sealed and bf16: the least factor on V costs it nothing."""
+    q_len, hq, hkv, kv_len, sealed = 900, 12, 2, 1000, 640
+    assert many(q_len, kv_len, hq, hkv)
+    q, data, scale, tail = T.make(dev, hq, hkv, q_len, kv_len, sealed, seed=1)
+    scale[1] *= 2.0 ** small
+    tail[1] = (tail[1].float() * 2.0 ** small).to(torch.bfloat16)
+    allowed = torch.ones(q_len, kv_len, dtype=torch.bool, device=dev)
     T.check(T.run(q, data, scale, tail, sealed, T.plan_of(allowed)),
             T.exact(q, data, scale, tail, sealed, allowed))
