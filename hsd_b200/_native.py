@@ -181,9 +181,10 @@ def ops():
             spec.loader.exec_module(module)
         except ImportError as e:
             raise HSDNativeError(f"cannot load {path}: {e}") from e
-        if module.built_for != ops_target():
-            raise HSDNativeError(f"{path} was built for {module.built_for}, this is "
-                                 f"{ops_target()}: rebuild it with `python -m hsd_b200.build`")
+        built_for = getattr(module, "built_for", "it does not say what")
+        if built_for != ops_target():
+            raise HSDNativeError(f"{path} was built for {built_for}, this is {ops_target()}: "
+                                 "rebuild it with `python -m hsd_b200.build`")
         _ops = module
     return _ops
 

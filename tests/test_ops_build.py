@@ -34,3 +34,20 @@ def test_another_versions_stamp_means_a_rebuild(monkeypatch, tmp_path):
     assert not B._ops_up_to_date()
     assert B._ops_command("x.so").count("-o") == 1
     assert any(N.ops_target() in a for a in B._ops_command("x.so"))
+
+
+def test_a_binding_that_does_not_say_is_refused(monkeypatch):
+    import importlib.machinery
+
+    class Loader:
+        def create_module(self, spec):
+            return None
+
+        def exec_module(self, module):
+            pass
+
+    monkeypatch.setattr(N, "_ops", None)
+    monkeypatch.setattr(N.importlib.util, "spec_from_file_location",
+                        lambda name, path: importlib.machinery.ModuleSpec(name, Loader()))
+    with pytest.raises(N.HSDNativeError, match="rebuild"):
+        N.ops()
